@@ -26,6 +26,7 @@ _TENSOR_OPS = [
     "relu_fwd", "relu_bwd", "relu_bwd_colsum", "add", "copy", "dropout", "rng_advance", "colsum",
     "maxpool_fwd", "maxpool_bwd", "maxpool_bwd_bn", "avgpool_fwd", "avgpool_bwd",
     "ce_loss", "adam_step", "sgd_step", "advance_step", "cast", "augment_mnist",
+    "group_norm_fwd", "group_norm_bwd", "linear_fprop", "linear_dgrad", "linear_wgrad", "adamw_step", "adamw8_step",
 ]
 
 
@@ -45,6 +46,7 @@ def _make(name):
 for _n in _TENSOR_OPS:
     globals()[_n] = _make(_n)
 
+adamw8_encode, adamw8_decode = ref_ops.adamw8_encode, ref_ops.adamw8_decode
 CompactAddendUnsupported = ref_ops.CompactAddendUnsupported
 SecondBnUnsupported = ref_ops.SecondBnUnsupported
 out_size = ref_ops.out_size

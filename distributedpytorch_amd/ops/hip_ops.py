@@ -302,6 +302,10 @@ def cast(src, dst):
     return dst
 
 
+from .hip_train_ops import (adamw8_step, adamw_step, group_norm_bwd, group_norm_fwd, linear_dgrad, linear_fprop,  # noqa: E402,F401
+                            linear_wgrad)
+
+
 # ----------------------------------------------------------------------------------------- input pipeline
 def augment_mnist(images, labels, index, out, labels_out, train, mean, std, seed, epoch):
     p = AugP()

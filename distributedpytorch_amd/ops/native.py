@@ -66,11 +66,28 @@ def lib_path(name: str) -> str:
 # entry points whose int return value is NOT a launch status (sizes, counts, modes) or is checked by its own caller
 _NOT_LAUNCH = {"dpa_conv_params_size", "dpa_wgrad_params_size", "dpa_pool_params_size", "dpa_aug_params_size",
                "dpa_bn_slab_rows", "dpa_conv_stats_rows", "dpa_conv_wgrad_workspace", "dpa_get_fp32_mode",
-               "dpa_set_fp32_mode", "dpa_x6p_min_tiles", "dpa_x6p_knob", "dpa_wgrad_knob", "dpa_x6s_knob", "dpa_maxpool_bwd_bn", "dpa_x6p_plausible", "dpa_weight_prep_seg_size", "dpa_conv_igemm", "dpa_conv_wgrad", "dpa_init_workspaces"}
+               "dpa_set_fp32_mode", "dpa_x6p_min_tiles", "dpa_x6p_knob", "dpa_wgrad_knob", "dpa_x6s_knob", "dpa_maxpool_bwd_bn", "dpa_x6p_plausible", "dpa_weight_prep_seg_size", "dpa_conv_igemm", "dpa_conv_wgrad", "dpa_init_workspaces",
+               "dpa_gn_params_size", "dpa_lin_params_size"}
 
 
 class KernelLaunchError(RuntimeError):
     pass
+
+
+class _OnDevice:
+    """Launches go to the tensors' device and its current stream, also while another device is the current one."""
+
+    def __init__(self, t):
+        self._guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return stream_ptr()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
 
 
 class _CheckedLib:

@@ -501,3 +501,326 @@ def augment_mnist(images, labels, index, out, labels_out, train, mean, std, seed
     out.zero_()
     out[..., :3] = res.unsqueeze(-1).to(out.dtype)
     return out
+
+
+# ----------------------------------------------------------------------------------------- group norm
+def _act(u, act):
+    if act == "relu":
+        return torch.relu(u)
+    if act == "silu":
+        return u * torch.sigmoid(u)
+    if act == "gelu":
+        return 0.5 * u * (1 + torch.erf(u * math.sqrt(0.5)))
+    return u
+
+
+def _act_slope(u, act):
+    if act == "relu":
+        return (u > 0).to(u.dtype)
+    if act == "silu":
+        s = torch.sigmoid(u)
+        return s * (1 + u * (1 - s))
+    if act == "gelu":
+        return 0.5 * (1 + torch.erf(u * math.sqrt(0.5))) + u * torch.exp(-0.5 * u * u) / math.sqrt(2 * math.pi)
+    return torch.ones_like(u)
+
+
+def _grouped(t, groups):
+    n, h, w, c = t.shape
+    return t.reshape(n, h * w, groups, c // groups)
+
+
+def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", residual=None):
+    """y = act((x - mean) * rstd * gamma + beta (+ residual)) for x [N, H, W, C] (fp32 or bf16, channel slices allowed), with
+    the mean and 1 / sqrt(variance + eps) of each image's groups of C / groups channels, which are left in mean and rstd
+    (fp32 [N, groups]) for the backward pass.  gamma, beta: fp32 [C].  act: "none", "relu", "silu" or "gelu".  y may be x
+    or residual itself."""
+    from . import checks
+    checks.group_norm("group_norm_fwd", x, gamma, beta, groups, mean, rstd)
+    checks.act_id(act)
+    checks.nhwc(y, "group_norm_fwd: y", x.shape, x.dtype)
+    if residual is not None:
+        checks.nhwc(residual, "group_norm_fwd: residual", x.shape, x.dtype)
+    checks.same_device("group_norm_fwd", x, y=y, residual=residual)
+    checks.overlap("group_norm_fwd", y, x=x, residual=residual)
+    if x.numel() == 0:
+        return y
+    t = _grouped(x.float(), groups)
+    mu = t.mean((1, 3))
+    d = t - mu[:, None, :, None]
+    rs = torch.rsqrt((d * d).mean((1, 3)) + eps)
+    u = (d * rs[:, None, :, None]).reshape(x.shape) * gamma + beta
+    if residual is not None:
+        u = u + residual.float()
+    mean.copy_(mu.view(mean.shape))
+    rstd.copy_(rs.view(rstd.shape))
+    y.copy_(_act(u, act))
+    return y
+
+
+def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbeta=None, act="none", y=None, residual=None,
+                   dresidual=None):
+    """Gradients of group_norm_fwd: dx, dgamma and dbeta (fp32 [C], or None where they are not wanted) and dresidual (or
+    None).  The activation's derivative is taken at values recomputed from x (and residual); for "relu" the stored output
+    may be given as y instead, its sign is then the mask.  dx may be dy or x itself, dresidual may be dy, y or residual."""
+    from . import checks
+    check_group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
+    if x.numel() == 0:
+        for t in (dgamma, dbeta):
+            if t is not None:
+                t.zero_()
+        return dx
+    mu, rs = mean.reshape(x.shape[0], 1, groups, 1), rstd.reshape(x.shape[0], 1, groups, 1)
+    xhat = (_grouped(x.float(), groups) - mu) * rs
+    dz = dy.float()
+    if act == "relu" and y is not None:
+        dz = dz * (y > 0)
+    elif act == "relu":
+        u = ((_grouped(x.double(), groups) - mu) * rs.double()).reshape(x.shape) * gamma.double() + beta
+        dz = dz * ((u if residual is None else u + residual) > 0)
+    elif act != "none":
+        u = xhat.reshape(x.shape) * gamma + beta
+        dz = dz * _act_slope(u if residual is None else u + residual.float(), act)
+    t = _grouped(dz * gamma, groups)
+    out = rs * (t - t.mean((1, 3), keepdim=True) - xhat * (t * xhat).mean((1, 3), keepdim=True))
+    if dgamma is not None:
+        dgamma.copy_((_grouped(dz, groups) * xhat).sum((0, 1)).reshape(-1))
+    if dbeta is not None:
+        dbeta.copy_(dz.sum((0, 1, 2)))
+    if dresidual is not None:
+        dresidual.copy_(dz)
+    dx.copy_(out.reshape(x.shape))
+    return dx
+
+
+def check_group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual):
+    """Channel strides (x, dy, dx, y, residual, dresidual), 0 for what is absent."""
+    from . import checks
+    name = "group_norm_bwd"
+    cs = [checks.group_norm(name, x, gamma, beta, groups, mean, rstd)]
+    checks.act_id(act)
+    for k, t in (("dy", dy), ("dx", dx), ("y", y), ("residual", residual), ("dresidual", dresidual)):
+        cs.append(0 if t is None else checks.nhwc(t, f"{name}: {k}", x.shape, x.dtype))
+    if y is not None and act != "relu":
+        raise ValueError(f"{name}: y is the mask of a ReLU; act is {act!r}")
+    for k, t in (("dgamma", dgamma), ("dbeta", dbeta)):
+        if t is not None:
+            checks.vec32(t, f"{name}: {k}", x.shape[3])
+    checks.same_device(name, x, dy=dy, dx=dx, y=y, residual=residual, dresidual=dresidual, dgamma=dgamma, dbeta=dbeta)
+    checks.overlap(name, dx, dy=dy, x=x, y=y, residual=residual)
+    if dresidual is not None:
+        checks.overlap(name, dresidual, dy=dy, y=y, residual=residual)
+        for k, t in (("x", x), ("dx", dx)):          # x is read again after dresidual was written
+            if dresidual.data_ptr() == t.data_ptr() and x.numel():
+                raise ValueError(f"{name}: dresidual may not be {k}")
+        checks.overlap(name, dresidual, x=x, dx=dx)
+    return cs
+
+
+# ----------------------------------------------------------------------------------------- linear products
+def check_linear_fprop(x, w, y, bias, act, addend, preact):
+    """Row strides (x, w, y, addend, preact)."""
+    from . import checks
+    name = "linear_fprop"
+    if x.dtype not in checks.FLOATS:
+        raise ValueError(f"{name}: x must be fp32 or bf16, got {x.dtype}")
+    ld = [checks.mat(x, f"{name}: x"), checks.mat(w, f"{name}: w", None, x.shape[1], x.dtype)]
+    m, n = x.shape[0], w.shape[0]
+    checks.act_id(act)
+    for k, t in (("y", y), ("addend", addend), ("preact", preact)):
+        ld.append(0 if t is None else checks.mat(t, f"{name}: {k}", m, n, x.dtype))
+    if n < 1 or x.shape[1] < 1:
+        raise ValueError(f"{name}: weight of shape {tuple(w.shape)}")
+    checks.matrix_dims(name, m, n, x.shape[1])
+    if bias is not None:
+        checks.vec32(bias, f"{name}: bias", n)
+    checks.same_device(name, x, w=w, y=y, bias=bias, addend=addend, preact=preact)
+    checks.overlap(name, y, addend=addend)
+    for k, o in (("y", y), ("preact", preact)):
+        for j, t in (("x", x), ("w", w)):
+            if o is not None and o.numel() and t.numel() and o.data_ptr() == t.data_ptr():
+                raise ValueError(f"{name}: {k} may not be {j}")
+            if o is not None:
+                checks.overlap(name, o, **{j: t})
+    if preact is not None:
+        checks.overlap(name, preact, addend=addend, y=y)
+        if preact.numel() and preact.data_ptr() == y.data_ptr():
+            raise ValueError(f"{name}: preact may not be y")
+    return ld
+
+
+def check_linear_dgrad(dy, w, dx, act, preact, addend):
+    """Row strides (dy, w, dx, preact, addend)."""
+    from . import checks
+    name = "linear_dgrad"
+    if dy.dtype not in checks.FLOATS:
+        raise ValueError(f"{name}: dy must be fp32 or bf16, got {dy.dtype}")
+    ld = [checks.mat(dy, f"{name}: dy"), checks.mat(w, f"{name}: w", dy.shape[1], None, dy.dtype)]
+    m, k = dy.shape[0], w.shape[1]
+    if checks.act_id(act) and preact is None:
+        raise ValueError(f"{name}: act {act!r} needs preact")
+    if not checks.act_id(act) and preact is not None:
+        raise ValueError(f"{name}: preact without an activation")
+    for key, t in (("dx", dx), ("preact", preact), ("addend", addend)):
+        ld.append(0 if t is None else checks.mat(t, f"{name}: {key}", m, k, dy.dtype))
+    if k < 1 or dy.shape[1] < 1:
+        raise ValueError(f"{name}: weight of shape {tuple(w.shape)}")
+    checks.matrix_dims(name, m, k, dy.shape[1])
+    checks.same_device(name, dy, w=w, dx=dx, preact=preact, addend=addend)
+    checks.overlap(name, dx, preact=preact, addend=addend)
+    for key, t in (("dy", dy), ("w", w)):
+        if dx.numel() and t.numel() and dx.data_ptr() == t.data_ptr():
+            raise ValueError(f"{name}: dx may not be {key}")
+        checks.overlap(name, dx, **{key: t})
+    return ld
+
+
+def check_linear_wgrad(dy, x, dw, db):
+    """Row strides (dy, x, dw)."""
+    from . import checks
+    name = "linear_wgrad"
+    if dy.dtype not in checks.FLOATS:
+        raise ValueError(f"{name}: dy must be fp32 or bf16, got {dy.dtype}")
+    ld = [checks.mat(dy, f"{name}: dy"), checks.mat(x, f"{name}: x", dy.shape[0], None, dy.dtype)]
+    n, k = dy.shape[1], x.shape[1]
+    if n < 1 or k < 1:
+        raise ValueError(f"{name}: no columns ({tuple(dy.shape)}, {tuple(x.shape)})")
+    ld.append(checks.mat(dw, f"{name}: dw", n, k, torch.float32))
+    checks.matrix_dims(name, n, k, dy.shape[0])
+    if db is not None:
+        checks.vec32(db, f"{name}: db", n)
+    checks.same_device(name, dy, x=x, dw=dw, db=db)
+    for key, t in (("dy", dy), ("x", x), ("db", db)):
+        if t is not None and t.numel() and dw.data_ptr() == t.data_ptr():
+            raise ValueError(f"{name}: dw may not be {key}")
+        checks.overlap(name, dw, **{key: t})
+    return ld
+
+
+def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
+    """y = act(x W^T + bias + addend) for x [M, in] and w [out, in] (both fp32 or both bf16, rows of any stride), bias fp32
+    [out].  preact receives the value in front of the activation, which linear_dgrad of the layer behind takes.  y or
+    preact may be addend itself."""
+    check_linear_fprop(x, w, y, bias, act, addend, preact)
+    u = x.float() @ w.float().t()
+    if bias is not None:
+        u = u + bias
+    if addend is not None:
+        u = u + addend.float()
+    if preact is not None:
+        preact.copy_(u)
+    y.copy_(_act(u, act))
+    return y
+
+
+def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
+    """dx = (dy W + addend) * act'(preact) for dy [M, out] and w [out, in]: the gradient in front of the activation whose
+    output was this layer's input, with the gradients that other readers of it left in addend.  dx may be addend or preact
+    itself."""
+    check_linear_dgrad(dy, w, dx, act, preact, addend)
+    d = dy.float() @ w.float()
+    if addend is not None:
+        d = d + addend.float()
+    if act != "none":
+        d = d * _act_slope(preact.float(), act)
+    dx.copy_(d)
+    return dx
+
+
+def linear_wgrad(dy, x, dw, db=None, accumulate=False):
+    """dw = dy^T x (fp32 [out, in]) and db = the column sums of dy (fp32 [out]); accumulate adds to what they hold."""
+    check_linear_wgrad(dy, x, dw, db)
+    w, b = dy.float().t() @ x.float(), dy.float().sum(0)
+    if accumulate:
+        dw.add_(w)
+        if db is not None:
+            db.add_(b)
+    else:
+        dw.copy_(w)
+        if db is not None:
+            db.copy_(b)
+    return dw
+
+
+# ----------------------------------------------------------------------------------------- AdamW
+def _adamw_update(p, g, m, v, p16, hyper, groups, group_ids, lo, hi):
+    h = [float(x) for x in hyper]
+    lr, b1, b2, eps, wd, step, _, gs, omb1, omb2 = h[:10]
+    b1d, b2d = b1 + h[10], b2 + h[11]
+    per = groups[group_ids[lo // 64: hi // 64].long()].repeat_interleave(64, 0)
+    gr = g[lo:hi] * gs
+    m = m + omb1 * (gr - m)
+    v = b2 * v + omb2 * gr * gr
+    step += 1
+    lrs = lr * per[:, 0]
+    denom = v.sqrt() / math.sqrt(1 - b2d ** step) + eps
+    p[lo:hi] = p[lo:hi] * (1 - lrs * (wd * per[:, 1])) - lrs / (1 - b1d ** step) * (m / denom)
+    if p16 is not None:
+        p16[lo:hi].copy_(p[lo:hi])
+    return m, v
+
+
+def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
+    """AdamW (decay decoupled from the gradient) on the range [lo, hi) of an arena whose tensors start at multiples of 64
+    elements.  hyper: nn/optim.py make_hyper, whose lr and weight decay are multiplied by the two entries of
+    groups[group_ids[i]] (fp32 [rows, 2]; uint8, one for each 64 elements).  p16: the bf16 compute copy, or None."""
+    from . import checks
+    n = p.numel()
+    hi = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi,
+                      {"m": (m, torch.float32, n), "v": (v, torch.float32, n)})
+    m[lo:hi], v[lo:hi] = _adamw_update(p, g, m[lo:hi].clone(), v[lo:hi].clone(), p16, hyper, groups, group_ids, lo, hi)
+
+
+ADAMW8_FORMATS = {"m": (torch.float8_e4m3fn, 448.0, -6, 3), "v": (torch.float8_e5m2, 57344.0, -14, 2)}
+
+
+def adamw8_random(seed, step, lo, hi, device):
+    """The two 16-bit random numbers of each element of a step: the finalizer of MurmurHash3 (Appleby) over the element's
+    index and a key made of seed and step."""
+    mask = 0xFFFFFFFF
+
+    def mix(h):
+        h = h ^ (h >> 16)
+        h = (h * 0x85EBCA6B) & mask
+        h = h ^ (h >> 13)
+        h = (h * 0xC2B2AE35) & mask
+        return h ^ (h >> 16)
+    key = mix(torch.tensor((seed + int(step) * 0x9E3779B9) & mask, device=device))
+    i = torch.arange(lo, hi, device=device)
+    h = mix((i & mask) ^ key ^ (((i >> 32) * 0x85EBCA6B) & mask))
+    return h & 0xFFFF, h >> 16
+
+
+def adamw8_encode(t, u, which):
+    """(codes, scales) of fp32 values in blocks of 64: 8-bit floats times one scale, rounded up with the probability of the
+    remainder (u: uniform numbers in (0, 1); 0.5 rounds to nearest).  csrc/hip/adamw.hip says why."""
+    dtype, top, least, bits = ADAMW8_FORMATS[which]
+    b = t.reshape(-1, 64)
+    most = torch.where(torch.isfinite(b), b.abs(), torch.zeros_like(b)).amax(1, keepdim=True)
+    some = most >= 2.0 ** -100
+    y = torch.nan_to_num(b.abs() * torch.where(some, top / most, torch.zeros_like(most)), nan=top, posinf=top).clamp_max(top)
+    e = (torch.frexp(y).exponent - 1).clamp_min(least)
+    q = torch.ldexp(torch.floor(torch.ldexp(y, bits - e) + u.reshape(b.shape)), e - bits).clamp_max(top)
+    if which == "v":
+        q = torch.where((b > 0) & some, q.clamp_min(2.0 ** (least - bits)), q)
+    return torch.copysign(q, b).reshape(-1).to(dtype), torch.where(some, most * (1.0 / top), torch.zeros_like(most)).reshape(-1)
+
+
+def adamw8_decode(codes, scales):
+    return codes.float() * scales.repeat_interleave(64)
+
+
+def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, seed, lo=0, hi=None):
+    """adamw_step with 8-bit states: m float8_e4m3fn, v float8_e5m2, one fp32 scale for each 64 elements (m_scale, v_scale),
+    rounded stochastically with numbers that depend on seed, the step in hyper and the element's index alone."""
+    n = p.numel()
+    from . import checks
+    hi = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
+                      {"m": (m, torch.float8_e4m3fn, n), "v": (v, torch.float8_e5m2, n),
+                       "m_scale": (m_scale, torch.float32, n // 64), "v_scale": (v_scale, torch.float32, n // 64)})
+    bl = slice(lo // 64, hi // 64)
+    mm, vv = _adamw_update(p, g, adamw8_decode(m[lo:hi], m_scale[bl]), adamw8_decode(v[lo:hi], v_scale[bl]), p16, hyper, groups,
+                           group_ids, lo, hi)
+    rm, rv = adamw8_random(seed, float(hyper[5]), lo, hi, p.device)
+    m[lo:hi], m_scale[bl] = adamw8_encode(mm, (rm.float() + 0.5) / 65536, "m")
+    v[lo:hi], v_scale[bl] = adamw8_encode(vv, (rv.float() + 0.5) / 65536, "v")
