@@ -1,0 +1,402 @@
+// Products of a linear layer with what surrounds them fused into the epilogue.
+//
+//   fprop   z = x W^T + bias (+ addend),  y = act(z)                x [M, K], W [N, K]; z is kept for the backward pass
+//   dgrad   dx = (dy W + addend) * act'(z)                          the derivative of the layer in FRONT, at its z [M, K]
+//   wgrad   dW = dy^T x,  db = column sums of dy
+//
+// All three are C[i, j] = sum_k A(i, k) B(j, k) of bf16 operands with fp32 accumulators; they differ in which index of an
+// operand is contiguous in memory: k (fprop: both; dgrad: dy) or i / j (dgrad: W; wgrad: both).
+// fp32 operands are taken as three bf16 parts, x = p0 + p1 + p2 exactly, and the product as the six largest part products
+// (the dropped ones are below 2^-23 of the term): the same kernel over six times the reduction, smallest terms first.
+#pragma once
+#include "act.h"
+#include "conv_common.h"
+#include <type_traits>
+
+struct LinParams {
+  const void *a, *b;                    // operands: bf16, row stride lda / ldb elements, parts a_part / b_part elements apart
+  long long lda, ldb, a_part, b_part;
+  const float* bias;                    // [cols]
+  const void *addend, *pre;             // pre: z of the activation whose derivative is multiplied in
+  void *out, *preact;
+  float* ws;                            // [splits][rows][cols] partial products where splits > 1
+  long long ld_add, ld_pre, ld_out, ld_z;
+  int rows, cols, K, parts, splits, accumulate, act, out32, vec, bias_vec;      // vec: every matrix of the epilogue takes 16-byte access
+};
+
+enum : int { EPI_FPROP = 0, EPI_DGRAD = 1, EPI_WGRAD = 2 };
+
+__device__ __attribute__((aligned(16))) const unsigned lin_zero[4] = {0, 0, 0, 0};
+
+// eight neighbouring elements of a row (n of them where the matrix ends or is not aligned: VEC = false)
+template <typename T> struct Lin8;
+template <> struct Lin8<bf16_t> {
+  uint4 w;
+  __device__ __forceinline__ float get(int e) const { const uint32_t u = ((const uint32_t*)&w)[e >> 1]; return __uint_as_float((e & 1) ? (u & 0xffff0000u) : (u << 16)); }
+  template <bool VEC> __device__ __forceinline__ void load(const bf16_t* p, int n) {
+    if (VEC) { w = *(const uint4*)p; return; }
+    uint32_t o[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (e < n) o[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+    w = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+};
+template <> struct Lin8<float> {
+  float4 a, b;
+  __device__ __forceinline__ float get(int e) const { return e < 4 ? ((const float*)&a)[e] : ((const float*)&b)[e - 4]; }
+  template <bool VEC> __device__ __forceinline__ void load(const float* p, int n) {
+    if (VEC) { a = *(const float4*)p; b = *(const float4*)(p + 4); return; }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { const float v = e < n ? p[e] : 0.f; if (e < 4) ((float*)&a)[e] = v; else ((float*)&b)[e - 4] = v; }
+  }
+};
+template <bool VEC> __device__ __forceinline__ void lin_st8(float* p, int n, const float (&v)[8]) {
+  if (VEC) { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]); return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < n) p[e] = v[e];
+}
+template <bool VEC> __device__ __forceinline__ void lin_st8(bf16_t* p, int n, const float (&v)[8]) {
+  if (VEC) {
+    uint4 o;
+    o.x = (uint32_t)f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16); o.y = (uint32_t)f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16);
+    o.z = (uint32_t)f2bf(v[4]) | ((uint32_t)f2bf(v[5]) << 16); o.w = (uint32_t)f2bf(v[6]) | ((uint32_t)f2bf(v[7]) << 16);
+    *(uint4*)p = o;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < n) p[e] = f2bf(v[e]);
+}
+
+// What is fused behind the product, for columns [j, j + n) of row i.  The reads are apart from the rest: an output may be one
+// of the inputs, so the compiler keeps loads behind stores, and a caller with several vectors reads for all of them first.
+template <typename T> struct LinExtra { Lin8<T> add, pre; };          // (wgrad: add = what is accumulated to)
+
+template <typename T, int EPI, int ACT, bool VEC>
+__device__ __forceinline__ void lin_extra(const LinParams& p, int i, int j, int n, LinExtra<T>& x) {
+  if (EPI == EPI_WGRAD) { if (p.accumulate) x.add.template load<VEC>((const T*)p.out + i * p.ld_out + j, n); return; }
+  if (p.addend) x.add.template load<VEC>((const T*)p.addend + i * p.ld_add + j, n);
+  if (EPI == EPI_DGRAD && ACT != ACT_NONE) x.pre.template load<VEC>((const T*)p.pre + i * p.ld_pre + j, n);
+}
+
+template <typename T, int EPI, int ACT, bool VEC>
+__device__ __forceinline__ void lin_finish(const LinParams& p, int i, int j, int n, const LinExtra<T>& x, const Lin8<float>& bias, float (&v)[8]) {
+  if (EPI == EPI_FPROP) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += bias.get(e);
+  }
+  if (EPI == EPI_WGRAD ? p.accumulate != 0 : p.addend != nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x.add.get(e);
+  }
+  if (EPI == EPI_FPROP) {
+    if (p.preact) lin_st8<VEC>((T*)p.preact + i * p.ld_z + j, n, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
+  } else if (EPI == EPI_DGRAD && ACT != ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= act_slope<ACT>(x.pre.get(e));
+  }
+  lin_st8<VEC>((T*)p.out + i * p.ld_out + j, n, v);
+}
+
+template <int EPI>
+__device__ __forceinline__ Lin8<float> lin_bias(const LinParams& p, int j, bool whole) {
+  Lin8<float> b;
+  b.a = b.b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (EPI == EPI_FPROP && p.bias && j < p.cols) { if (whole) b.load<true>(p.bias + j, 8); else b.load<false>(p.bias + j, p.cols - j); }
+  return b;
+}
+
+// calls f(std::integral_constant<int, ACT>, std::bool_constant<VEC>) for the launch's activation and alignment
+template <int EPI, typename F>
+__device__ __forceinline__ void lin_by_kind(const LinParams& p, F f) {
+  using std::integral_constant;
+  if (EPI == EPI_WGRAD) { if (p.vec) f(integral_constant<int, 0>(), std::true_type()); else f(integral_constant<int, 0>(), std::false_type()); return; }
+#define LIN_KIND(A) if (p.act == A) { if (p.vec) f(integral_constant<int, A>(), std::true_type()); else f(integral_constant<int, A>(), std::false_type()); return; }
+  LIN_KIND(ACT_NONE) LIN_KIND(ACT_RELU) LIN_KIND(ACT_SILU) LIN_KIND(ACT_GELU)
+#undef LIN_KIND
+}
+
+// ---- operand tiles in LDS ------------------------------------------------------------------------------------------------
+// A K step is 64 elements.  An operand tile of R rows (i or j) holds R x 64 bf16 in one of two layouts, both
+// written by the LDS DMA in pieces of 1 KiB (64 lanes x 16 bytes), the swizzle applied to the SOURCE address:
+//  k contiguous:   [R][64], 16-byte chunk c of row r at c ^ s(r): 16 rows x one chunk fall on 16 different bank groups.  A
+//                  fragment (lane l: row l & 15, 8 elements from k = 8 (l >> 4)) is one ds_read_b128.
+//  k strided (T):  [64][R], rows of R elements; a unit of 16 elements (32 bytes) u of row k at u ^ g(k).  A fragment is two
+//                  ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 elements and get them transposed.  g spreads the 8 rows that
+//                  32 lanes read over the 64 banks.
+template <int R> __device__ __forceinline__ int lin_g(int k) {
+  return R >= 128 ? (k & 3) | (((k >> 3) & 1) << 2) : ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
+}
+__device__ __forceinline__ int lin_s(int r) { return (r >> 1) & 7; }
+
+// source of one 16-byte chunk of a piece in this lane at K step 0 of part 0; k: the chunk's first k in the step
+template <int R, bool T>
+__device__ __forceinline__ const bf16_t* lin_source(const void* base, long long ld, int r0, int limit, int piece, int lane, int& k) {
+  if (!T) {
+    const int r = piece * 8 + (lane >> 3);
+    k = ((lane & 7) ^ lin_s(r)) * 8;
+    return (const bf16_t*)base + (long long)min(r0 + r, limit - 1) * ld + k;
+  }
+  constexpr int KPP = 512 / R, LPR = R / 8;              // rows of k in a piece, lanes per row
+  k = piece * KPP + lane / LPR;
+  const int slot = lane % LPR, e = r0 + (((slot >> 1) ^ lin_g<R>(k)) * 2 + (slot & 1)) * 8;
+  return (const bf16_t*)base + (long long)k * ld + (e < limit ? e : 0);
+}
+
+// One 16-row fragment of K part ks (32 elements).
+template <int R, bool T>
+__device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int lane) {
+  const int l15 = lane & 15, q4 = lane >> 4;
+  if (!T) return *(const bf16x8*)(t + (u * 16 + l15) * 128 + ((ks * 4 + q4) ^ lin_s(l15)) * 16);
+  const int k = ks * 32 + q4 * 8 + (l15 >> 2);
+  const char* a = t + k * (R * 2) + (u ^ lin_g<R>(k)) * 32 + (l15 & 3) * 8;
+  const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)a);
+  const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)(a + 4 * R * 2));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// this wave's pieces have landed and its LDS reads are done; behind the barrier, everyone's
+__device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The blocks are persistent and see ONE stream of K steps across their tiles: while step s is multiplied, step s + 1 lands, and
+// step s + 2 is requested as soon as the buffer of step s is free, also when it belongs to the next tile, so the epilogue of
+// a tile runs under the first loads of the next.  A step has four phases, each the matrix instructions of half the wave's
+// rows and half the step; a phase first reads the fragments of the NEXT phase from LDS.  The barrier stands before the last
+// phase: behind it everyone's reads of the buffer are done (registers hold what is left to multiply) and everyone's pieces
+// of step s + 1 have landed.
+template <typename T, int WM, int WN, int MT, int NT, int EPI>
+__global__ void __launch_bounds__(WM * WN * 64, 2) lin_mfma_kernel(LinParams p) {
+  constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
+  constexpr int BM = WM * MT * 16, BN = WN * NT * 16, NW = WM * WN, H = MT / 2;
+  constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
+  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // 1 KiB pieces a wave stages per step
+  static_assert(PA >= 1 && PB >= 1 && MT % 2 == 0 && MT <= 8 && NT % 2 == 0, "tile");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int tm = (p.rows + BM - 1) / BM, tn = (p.cols + BN - 1) / BN, tiles = tm * tn, jobs = tiles * p.splits;
+  const int ksteps = (p.K + 63) / 64, total = ksteps * (p.parts == 1 ? 1 : 6), per = (total + p.splits - 1) / p.splits;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
+
+  // blocks of one XCD get neighbouring tiles: panels of 8 tile rows, walked column by column
+  auto place = [&](int job, int& i0, int& j0, int& split) {
+    const int id = xcd_remap(job, jobs);
+    split = id / tiles;
+    const int tile = id - split * tiles, panel = tile / (8 * tn), in = tile - panel * 8 * tn, ph = min(8, tm - panel * 8);
+    i0 = (panel * 8 + in % ph) * BM; j0 = (in / ph) * BN;
+  };
+
+  // ---- the stream of requests
+  const bf16_t* ap[PA]; const bf16_t* bp[PB];
+  int ak[PA], bk[PB];
+  int d_job = blockIdx.x, d_kt = 0, d_end = 0;
+  auto d_place = [&]() {
+    int i0, j0, split;
+    place(d_job, i0, j0, split);
+    d_kt = split * per; d_end = min(d_kt + per, total);
+#pragma unroll
+    for (int q = 0; q < PA; ++q) ap[q] = lin_source<BM, AT>(p.a, p.lda, i0, p.rows, wave * PA + q, lane, ak[q]);
+#pragma unroll
+    for (int q = 0; q < PB; ++q) bp[q] = lin_source<BN, BT>(p.b, p.ldb, j0, p.cols, wave * PB + q, lane, bk[q]);
+  };
+  auto request = [&](int to) __attribute__((always_inline)) {
+    if (d_job >= jobs) return;
+    const int seg = p.parts == 1 ? 0 : d_kt / ksteps, ks = d_kt - seg * ksteps;
+    // parts of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+    const int pa = p.parts == 1 ? 0 : (0x001102 >> (seg * 4)) & 15, pb = p.parts == 1 ? 0 : (0x010120 >> (seg * 4)) & 15;
+    const long long oa = pa * p.a_part + (AT ? ks * 64 * p.lda : (long long)ks * 64);
+    const long long ob = pb * p.b_part + (BT ? ks * 64 * p.ldb : (long long)ks * 64);
+    const int left = p.K - ks * 64;
+    const uint32_t stage = lds0 + to * STAGE;
+    if (left < 64) {          // the last step of an odd reduction: zeros behind its end
+#pragma unroll
+      for (int q = 0; q < PA; ++q) dpa_glds16(ak[q] < left ? ap[q] + oa : (const bf16_t*)lin_zero, stage + (wave * PA + q) * 1024);
+#pragma unroll
+      for (int q = 0; q < PB; ++q) dpa_glds16(bk[q] < left ? bp[q] + ob : (const bf16_t*)lin_zero, stage + A_BYTES + (wave * PB + q) * 1024);
+    } else {
+#pragma unroll
+      for (int q = 0; q < PA; ++q) dpa_glds16(ap[q] + oa, stage + (wave * PA + q) * 1024);
+#pragma unroll
+      for (int q = 0; q < PB; ++q) dpa_glds16(bp[q] + ob, stage + A_BYTES + (wave * PB + q) * 1024);
+    }
+    if (++d_kt == d_end) { d_job += gridDim.x; if (d_job < jobs) d_place(); }
+  };
+
+  f32x4 acc[MT][NT];
+  bf16x8 fa[MT], fb[2][NT];
+  auto read_a = [&](int buf, int half, int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) fa[half * H + i] = lin_fragment<BM, AT>(smem + buf * STAGE, wm * MT + half * H + i, ks, lane);
+  };
+  auto read_b = [&](int buf, int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fb[ks][j] = lin_fragment<BN, BT>(smem + buf * STAGE + A_BYTES, wn * NT + j, ks, lane);
+  };
+  auto multiply = [&](int half, int ks) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)          // (j rows, i columns: a lane then holds four neighbouring columns of one output row)
+        acc[half * H + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[ks][j], fa[half * H + i], acc[half * H + i][j], 0, 0, 0);
+  };
+
+  d_place();
+  request(0);
+  request(1);
+  lin_sync();
+  int buf = 0;
+  for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+    int i0, j0, split;
+    place(job, i0, j0, split);
+    const int kt0 = split * per, kt1 = min(kt0 + per, total);
+    read_b(buf, 0);
+    read_a(buf, 0, 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int kt = kt0; kt < kt1; ++kt) {
+      read_a(buf, 1, 0);
+      multiply(0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_b(buf, 1);
+      read_a(buf, 0, 1);
+      multiply(1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      read_a(buf, 1, 1);
+      multiply(0, 1);
+      lin_sync();
+      request(buf);
+      buf ^= 1;
+      if (kt + 1 < kt1) {
+        read_b(buf, 0);
+        read_a(buf, 0, 0);
+      }
+      multiply(1, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // ---- epilogue, from registers.  Neighbouring 16-column tiles trade quarters, so that a lane holds 8 columns of one row,
+    // and the lanes are permuted so that four neighbouring ones hold 32 neighbouring columns: 64-byte requests instead of
+    // 16-byte ones, each of which would take the address unit as long.
+    // One row tile at a time in a rolled loop (the code of an activation is long); the accumulators are picked by a scalar
+    // branch.  What bf16 epilogues read is requested one trip ahead.
+    const int from = ((((lane & 1) << 1) | ((lane >> 1) & 1)) * 16 + (lane >> 2)) * 4;
+    constexpr int NV = NT / 2;      // vectors of 8 columns a lane finishes in a trip
+    auto where = [&](int i, int k, int& gi, int& gj) __attribute__((always_inline)) {
+      gi = i0 + (wm * MT + i) * 16 + (lane >> 2);
+      gj = j0 + (wn * NT + k * 2) * 16 + (lane & 3) * 8;
+      return gi < p.rows && gj < p.cols;
+    };
+    auto trips = [&](auto before, auto finish) __attribute__((always_inline)) {
+      before(0);
+#pragma unroll 1
+      for (int i = 0; i < MT; ++i) {
+        f32x4 t[NT];
+        switch (i) {
+#define LIN_PICK(I) case I: for (int j = 0; j < NT; ++j) t[j] = acc[I < MT ? I : 0][j]; break;
+          LIN_PICK(0) LIN_PICK(1) LIN_PICK(2) LIN_PICK(3) LIN_PICK(4) LIN_PICK(5) LIN_PICK(6) LIN_PICK(7)
+#undef LIN_PICK
+        }
+        float v[NV][8];
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(t[2 * k][e]), __float_as_uint(t[2 * k + 1][e]), false, false);
+            v[k][e] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, w[0]));
+            v[k][e + 4] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, w[1]));
+          }
+        finish(i, v);
+      }
+    };
+    int gi, gj;
+    if (p.splits > 1) {
+      float* ws = p.ws + (long long)split * p.rows * p.cols;
+      const bool vec = (p.cols & 7) == 0;
+      trips([](int) {}, [&](int i, float (&v)[NV][8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          if (where(i, k, gi, gj)) {
+            float* o = ws + (long long)gi * p.cols + gj;
+            if (vec) lin_st8<true>(o, 8, v[k]); else lin_st8<false>(o, min(8, p.cols - gj), v[k]);
+          }
+      });
+    } else {
+      lin_by_kind<EPI>(p, [&](auto act, auto vec) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(act)::value;
+        constexpr bool VEC = decltype(vec)::value, AHEAD = sizeof(T) == 2 && VEC;
+        LinExtra<T> x[NV], y[NV];
+        Lin8<float> bias[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) { where(0, k, gi, gj); bias[k] = lin_bias<EPI>(p, gj, p.bias_vec); }
+        auto load = [&](int i, LinExtra<T> (&to)[NV]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int k = 0; k < NV; ++k)
+            if (where(i, k, gi, gj)) lin_extra<T, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), to[k]);
+        };
+        trips([&](int i) __attribute__((always_inline)) { if (AHEAD) load(i, y); },
+              [&](int i, float (&v)[NV][8]) __attribute__((always_inline)) {
+                if (AHEAD) {
+#pragma unroll
+                  for (int k = 0; k < NV; ++k) x[k] = y[k];
+                  if (i + 1 < MT) load(i + 1, y);
+                } else {
+                  load(i, x);
+                }
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+                  if (where(i, k, gi, gj)) lin_finish<T, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), x[k], bias[k], v[k]);
+              });
+      });
+    }
+  }
+}
+
+// joins the partial products of a split reduction in a fixed order and applies the epilogue
+template <typename T, int EPI>
+__global__ void __launch_bounds__(256) lin_join_kernel(LinParams p) {
+  const int groups = (p.cols + 7) / 8;
+  const long long total = (long long)p.rows * groups, part = (long long)p.rows * p.cols;
+  const bool whole = (p.cols & 7) == 0;
+  for (long long t = blockIdx.x * 256LL + threadIdx.x; t < total; t += gridDim.x * 256LL) {
+    const int i = (int)(t / groups), j = (int)(t - (long long)i * groups) * 8, n = min(8, p.cols - j);
+    float v[8] = {};
+    for (int k = 0; k < p.splits; ++k) {
+      Lin8<float> s;
+      const float* w = p.ws + k * part + (long long)i * p.cols + j;
+      if (whole) s.load<true>(w, 8); else s.load<false>(w, n);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += s.get(e);
+    }
+    lin_by_kind<EPI>(p, [&](auto act, auto vec) {
+      LinExtra<T> x;
+      lin_extra<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x);
+      lin_finish<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x, lin_bias<EPI>(p, j, p.bias_vec), v);
+    });
+  }
+}
+
+template <typename T, int WM, int WN, int MT, int NT, int EPI>
+static int lin_run(const LinParams& p, hipStream_t s) {
+  constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
+  constexpr int lds = 2 * (BM + BN) * 128, residents = 160 * 1024 / lds;
+  const long long jobs = (long long)((p.rows + BM - 1) / BM) * ((p.cols + BN - 1) / BN) * p.splits;
+  if (jobs > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+  static const int once = (int)hipFuncSetAttribute((const void*)lin_mfma_kernel<T, WM, WN, MT, NT, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (once) return once;
+  const int grid = (int)(jobs < 256 * residents ? jobs : 256 * residents);      // (a multiple of 8 where there are several rounds: xcd_remap)
+  lin_mfma_kernel<T, WM, WN, MT, NT, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
+  if (p.splits > 1) lin_join_kernel<T, EPI><<<dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256), 256, 0, s>>>(p);
+  return dpa_launch_rc();
+}
+
+template <typename T, int EPI>
+static int lin_tile(const LinParams& p, int tile, hipStream_t s) {
+  switch (tile) {
+    case 0: return lin_run<T, 2, 4, 8, 4, EPI>(p, s);      // 256 x 256, 8 waves
+    case 1: return lin_run<T, 2, 2, 4, 4, EPI>(p, s);      // 128 x 128, 4 waves
+    case 2: return lin_run<T, 2, 2, 2, 2, EPI>(p, s);      // 64 x 64, 4 waves
+  }
+  return (int)hipErrorInvalidValue;
+}

@@ -1,67 +1,44 @@
-// Products of a linear layer with what surrounds them fused into the epilogue.
-//
-//   fprop   z = x W^T + bias (+ addend),  y = act(z)                x [M, K], W [N, K]; z is kept for the backward pass
-//   dgrad   dx = (dy W + addend) * act'(z)                          the derivative of the layer in FRONT, at its z [M, K]
-//   wgrad   dW = dy^T x,  db = column sums of dy
-#include "act.h"
+// Entry points of the linear products (linear.h), the operand packing and the bias gradient.
+#include "linear.h"
 
-struct LinParams {
-  const void *a, *b;                    // C[i, j] = sum_k A(i, k) B(j, k)
-  long long a_i, a_k, b_j, b_k;         // element strides
-  const float* bias;                    // [cols]
-  const void *addend, *pre;             // pre: z of the activation whose derivative is multiplied in
-  void *out, *preact;
-  long long ld_add, ld_pre, ld_out, ld_z;
-  int rows, cols, K, accumulate;
-};
+int lin_fprop(const LinParams& p, int tile, hipStream_t s);
+int lin_dgrad(const LinParams& p, int tile, hipStream_t s);
+int lin_wgrad(const LinParams& p, int tile, hipStream_t s);
 
-enum : int { EPI_FPROP = 0, EPI_DGRAD = 1, EPI_WGRAD = 2 };
-
-template <typename T, int EPI, int ACT>
-__device__ __forceinline__ void lin_store(const LinParams& p, int i, int j, float v) {
-  if (EPI == EPI_WGRAD) {
-    float* o = (float*)p.out + i * p.ld_out + j;
-    *o = p.accumulate ? *o + v : v;
-    return;
-  }
-  if (EPI == EPI_FPROP && p.bias) v += p.bias[j];
-  if (p.addend) v += Elem<T>::ld((const T*)p.addend + i * p.ld_add + j);
-  if (EPI == EPI_FPROP) {
-    if (p.preact) Elem<T>::st((T*)p.preact + i * p.ld_z + j, v);
-    v = act_fwd<ACT>(v);
-  } else if (ACT != ACT_NONE) {
-    v *= act_slope<ACT>(Elem<T>::ld((const T*)p.pre + i * p.ld_pre + j));
-  }
-  Elem<T>::st((T*)p.out + i * p.ld_out + j, v);
-}
-
-// 64 x 64 tile, 4 x 4 outputs a thread, any strides
-template <typename T, int EPI, int ACT>
-__global__ void __launch_bounds__(256) lin_simple_kernel(LinParams p) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int t = threadIdx.x, tx = t & 15, ty = t >> 4, i0 = blockIdx.x * 64;
-  for (int j0 = blockIdx.y * 64; j0 < p.cols; j0 += gridDim.y * 64) {
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 16) {
-      for (int e = t; e < 1024; e += 256) {
-        const int r = e >> 4, k = e & 15;
-        sa[k][r] = (i0 + r < p.rows && k0 + k < p.K) ? Elem<T>::ld((const T*)p.a + (i0 + r) * p.a_i + (k0 + k) * p.a_k) : 0.f;
-        sb[k][r] = (j0 + r < p.cols && k0 + k < p.K) ? Elem<T>::ld((const T*)p.b + (j0 + r) * p.b_j + (k0 + k) * p.b_k) : 0.f;
+// ---- operands that the DMA cannot take as they are -----------------------------------------------------------------------
+// fp32 matrices become their three bf16 parts, bf16 matrices with odd rows or addresses a copy with rows of a multiple of 8;
+// the columns behind the last one are zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) lin_pack_kernel(const T* __restrict__ src, long long ld, int rows, int cols, int ldd, int vec,
+                                                       bf16_t* __restrict__ dst) {
+  const int groups = ldd / 8;
+  const long long total = (long long)rows * groups, part = (long long)rows * ldd;
+  for (long long t = blockIdx.x * 256LL + threadIdx.x; t < total; t += gridDim.x * 256LL) {
+    const int i = (int)(t / groups), j = (int)(t - (long long)i * groups) * 8;
+    Lin8<T> v;
+    if (vec && j + 8 <= cols) v.template load<true>(src + i * ld + j, 8); else v.template load<false>(src + i * ld + j, cols - j);
+    uint32_t o[3][4];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = v.get(e + h);
+        bf16_t b0 = f2bf(x);
+        if (sizeof(T) == 4) {
+          if ((b0 & 0x7FFF) == 0x7F80 && fabsf(x) < INFINITY) b0 = (bf16_t)(__float_as_uint(x) >> 16);      // no overflow by rounding
+          const bool fin = fabsf(x) < INFINITY;
+          const float r1 = fin ? x - bf2f(b0) : 0.f;
+          const bf16_t b1 = f2bf(r1), b2 = f2bf(r1 - bf2f(b1));
+          w[1] |= (uint32_t)b1 << (16 * h); w[2] |= (uint32_t)b2 << (16 * h);
+        }
+        w[0] |= (uint32_t)b0 << (16 * h);
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[r][c] += sa[k][ty * 4 + r] * sb[k][tx * 4 + c];
-      __syncthreads();
+      o[0][e / 2] = w[0]; o[1][e / 2] = w[1]; o[2][e / 2] = w[2];
     }
-    for (int r = 0; r < 4; ++r)
-      for (int c = 0; c < 4; ++c) {
-        const int i = i0 + ty * 4 + r, j = j0 + tx * 4 + c;
-        if (i < p.rows && j < p.cols) lin_store<T, EPI, ACT>(p, i, j, acc[r][c]);
-      }
+#pragma unroll
+    for (int q = 0; q < (sizeof(T) == 4 ? 3 : 1); ++q)
+      *(uint4*)(dst + q * part + (long long)i * ldd + j) = make_uint4(o[q][0], o[q][1], o[q][2], o[q][3]);
   }
 }
 
@@ -86,33 +63,21 @@ __global__ void __launch_bounds__(256) lin_colsum_join_kernel(const float* __res
   out[c] = accumulate ? out[c] + s : s;
 }
 
-template <typename T, int EPI, int ACT>
-static int lin_launch(const LinParams& p, hipStream_t s) {
-  const dim3 grid((p.rows + 63) / 64, min((p.cols + 63) / 64, 65535));
-  lin_simple_kernel<T, EPI, ACT><<<grid, 256, 0, s>>>(p);
-  return dpa_launch_rc();
-}
 
-template <typename T, int EPI>
-static int lin_by_act(const LinParams& p, int act, hipStream_t s) {
-  switch (act) {
-    case ACT_NONE: return lin_launch<T, EPI, ACT_NONE>(p, s);
-    case ACT_RELU: return lin_launch<T, EPI, ACT_RELU>(p, s);
-    case ACT_SILU: return lin_launch<T, EPI, ACT_SILU>(p, s);
-    case ACT_GELU: return lin_launch<T, EPI, ACT_GELU>(p, s);
+DPA_API int dpa_lin_params_size() { return (int)sizeof(LinParams); }
+DPA_API int dpa_linear(const LinParams* p, int epi, int tile, hipStream_t s) {
+  switch (epi) {
+    case EPI_FPROP: return lin_fprop(*p, tile, s);
+    case EPI_DGRAD: return lin_dgrad(*p, tile, s);
+    case EPI_WGRAD: return lin_wgrad(*p, tile, s);
   }
   return (int)hipErrorInvalidValue;
 }
-
-DPA_API int dpa_lin_params_size() { return (int)sizeof(LinParams); }
-DPA_API int dpa_linear_fprop(const LinParams* p, int act, int dtype, hipStream_t s) {
-  return dtype == 0 ? lin_by_act<float, EPI_FPROP>(*p, act, s) : lin_by_act<bf16_t, EPI_FPROP>(*p, act, s);
-}
-DPA_API int dpa_linear_dgrad(const LinParams* p, int act, int dtype, hipStream_t s) {
-  return dtype == 0 ? lin_by_act<float, EPI_DGRAD>(*p, act, s) : lin_by_act<bf16_t, EPI_DGRAD>(*p, act, s);
-}
-DPA_API int dpa_linear_wgrad(const LinParams* p, int dtype, hipStream_t s) {
-  return dtype == 0 ? lin_launch<float, EPI_WGRAD, ACT_NONE>(*p, s) : lin_launch<bf16_t, EPI_WGRAD, ACT_NONE>(*p, s);
+DPA_API int dpa_linear_pack(const void* src, long long ld, int rows, int cols, int ldd, int vec, void* dst, int dtype, hipStream_t s) {
+  const int grid = dpa_grid((long long)rows * (ldd / 8), 256);
+  if (dtype == 0) lin_pack_kernel<float><<<grid, 256, 0, s>>>((const float*)src, ld, rows, cols, ldd, vec, (bf16_t*)dst);
+  else lin_pack_kernel<bf16_t><<<grid, 256, 0, s>>>((const bf16_t*)src, ld, rows, cols, ldd, vec, (bf16_t*)dst);
+  return dpa_launch_rc();
 }
 DPA_API int dpa_linear_colsum(const void* x, long long ld, int rows, int cols, int splits, int per, float* slab, int accumulate, float* out,
                               int dtype, hipStream_t s) {

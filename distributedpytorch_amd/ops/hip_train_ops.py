@@ -21,9 +21,10 @@ class GnParams(ctypes.Structure):
 
 
 class LinParams(ctypes.Structure):
-    _fields_ = [("a", VP), ("b", VP), ("a_i", I64), ("a_k", I64), ("b_j", I64), ("b_k", I64), ("bias", VP), ("addend", VP), ("pre", VP),
-                ("out", VP), ("preact", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
-                ("rows", I32), ("cols", I32), ("K", I32), ("accumulate", I32)]
+    _fields_ = [("a", VP), ("b", VP), ("lda", I64), ("ldb", I64), ("a_part", I64), ("b_part", I64), ("bias", VP), ("addend", VP), ("pre", VP),
+                ("out", VP), ("preact", VP), ("ws", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
+                ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("out32", I32),
+                ("vec", I32), ("bias_vec", I32)]
 
 
 _checked = []
@@ -94,17 +95,69 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
 
 
 # ----------------------------------------------------------------------------------------- linear products
+_FPROP, _DGRAD, _WGRAD = 0, 1, 2          # csrc/hip/linear.hip
+_TILES = ((256, 256), (128, 128), (64, 64))
+
+
+def _plan(rows, cols, ksteps):
+    """(tile, splits of the reduction)"""
+    for i, (bm, bn) in enumerate(_TILES):
+        blocks = ((rows + bm - 1) // bm) * ((cols + bn - 1) // bn)
+        if blocks >= 200:
+            return i, 1
+    blocks = ((rows + 63) // 64) * ((cols + 63) // 64)
+    return 2, max(1, min(256 // blocks, ksteps // 4, 16))
+
+
+def _aligned(t, ld):
+    es = t.element_size()
+    return t.data_ptr() % 16 == 0 and (ld * es) % 16 == 0
+
+
+def _operand(t, ld, stream, keep):
+    """(pointer, row stride, stride of its parts, parts): the matrix as the kernel's DMA takes it - bf16 rows of a multiple
+    of 8 elements at 16-byte addresses as they are, anything else through lin_pack_kernel."""
+    rows, cols = t.shape
+    f32 = t.dtype == torch.float32
+    if not f32 and cols % 8 == 0 and _aligned(t, ld):
+        return ptr(t), ld, 0
+    ldd = (cols + 7) // 8 * 8
+    buf = torch.empty((3 if f32 else 1) * rows * ldd, device=t.device, dtype=torch.bfloat16)
+    keep.append(buf)
+    if rows:
+        _lib().dpa_linear_pack(ptr(t), I64(ld), rows, cols, ldd, int(_aligned(t, ld)), ptr(buf), _DT[t.dtype], stream)
+    return ptr(buf), ldd, rows * ldd
+
+
+def _product(epi, a, lda, b, ldb, p, k, stream, keep):
+    p.a, p.lda, p.a_part = _operand(a, lda, stream, keep)
+    p.b, p.ldb, p.b_part = _operand(b, ldb, stream, keep)
+    p.K, p.parts = k, 3 if a.dtype == torch.float32 else 1
+    tile, p.splits = _plan(p.rows, p.cols, (k + 63) // 64 * (6 if p.parts == 3 else 1))
+    if p.splits > 1:
+        ws = torch.empty(p.splits * p.rows * p.cols, device=a.device, dtype=torch.float32)
+        keep.append(ws)
+        p.ws = ptr(ws)
+    _lib().dpa_linear(ctypes.byref(p), epi, tile, stream)
+
+
+def _vec(cols, *mats):
+    return int(cols % 8 == 0 and all(t is None or _aligned(t, ld) for t, ld in mats))
+
+
 def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
     ldx, ldw, ldy, lda, ldz = ref_ops.check_linear_fprop(x, w, y, bias, act, addend, preact)
     if x.shape[0] == 0:
         return y
     p = LinParams()
-    p.a, p.b, p.a_i, p.a_k, p.b_j, p.b_k = ptr(x), ptr(w), ldx, 1, ldw, 1
     p.bias, p.addend, p.out, p.preact = ptr(bias), ptr(addend), ptr(y), ptr(preact)
     p.ld_add, p.ld_out, p.ld_z = lda, ldy, ldz
-    p.rows, p.cols, p.K = x.shape[0], w.shape[0], x.shape[1]
+    p.rows, p.cols, p.act, p.out32 = x.shape[0], w.shape[0], checks.act_id(act), int(x.dtype == torch.float32)
+    p.vec = _vec(p.cols, (y, ldy), (addend, lda), (preact, ldz))
+    p.bias_vec = int(bias is not None and p.cols % 8 == 0 and bias.data_ptr() % 16 == 0)
+    keep = []
     with _OnDevice(x) as stream:
-        _lib().dpa_linear_fprop(ctypes.byref(p), checks.act_id(act), _DT[x.dtype], stream)
+        _product(_FPROP, x, ldx, w, ldw, p, x.shape[1], stream, keep)
     return y
 
 
@@ -113,23 +166,25 @@ def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
     if dy.shape[0] == 0:
         return dx
     p = LinParams()
-    p.a, p.b, p.a_i, p.a_k, p.b_j, p.b_k = ptr(dy), ptr(w), ldy, 1, 1, ldw
     p.addend, p.pre, p.out = ptr(addend), ptr(preact), ptr(dx)
     p.ld_add, p.ld_pre, p.ld_out = lda, ldp, ldx
-    p.rows, p.cols, p.K = dy.shape[0], w.shape[1], dy.shape[1]
+    p.rows, p.cols, p.act, p.out32 = dy.shape[0], w.shape[1], checks.act_id(act), int(dy.dtype == torch.float32)
+    p.vec = _vec(p.cols, (dx, ldx), (addend, lda), (preact, ldp))
+    keep = []
     with _OnDevice(dy) as stream:
-        _lib().dpa_linear_dgrad(ctypes.byref(p), checks.act_id(act), _DT[dy.dtype], stream)
+        _product(_DGRAD, dy, ldy, w, ldw, p, dy.shape[1], stream, keep)
     return dx
 
 
 def linear_wgrad(dy, x, dw, db=None, accumulate=False):
     ldy, ldx, ldw = ref_ops.check_linear_wgrad(dy, x, dw, db)
     p = LinParams()
-    p.a, p.b, p.a_i, p.a_k, p.b_j, p.b_k = ptr(dy), ptr(x), 1, ldy, 1, ldx
     p.out, p.ld_out, p.accumulate = ptr(dw), ldw, int(accumulate)
-    p.rows, p.cols, p.K = dy.shape[1], x.shape[1], dy.shape[0]
+    p.rows, p.cols = dy.shape[1], x.shape[1]
+    p.vec = _vec(p.cols, (dw, ldw))
+    keep = []
     with _OnDevice(dy) as stream:
-        _lib().dpa_linear_wgrad(ctypes.byref(p), _DT[dy.dtype], stream)
+        _product(_WGRAD, dy, ldy, x, ldx, p, dy.shape[0], stream, keep)
         if db is not None:
             m, n = dy.shape
             splits = max(1, min((m + 63) // 64, 2048 // ((n + 63) // 64), 64))
