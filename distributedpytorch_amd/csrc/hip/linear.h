@@ -11,6 +11,7 @@
 #pragma once
 #include "act.h"
 #include "conv_common.h"
+#include <atomic>
 #include <type_traits>
 
 struct LinParams {
@@ -21,7 +22,17 @@ struct LinParams {
   void *out, *preact;
   float* ws;                            // [splits][rows][cols] partial products where splits > 1
   long long ld_add, ld_pre, ld_out, ld_z;
-  int rows, cols, K, parts, splits, accumulate, act, out32, vec, bias_vec;      // vec: every matrix of the epilogue takes 16-byte access
+  int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, pad;      // vec: every matrix of the epilogue takes 16-byte access
+};
+
+// What a call hands over besides: the operands as they are, what they are packed into first (ld 0: nothing), the bias gradient.
+struct LinCall {
+  LinParams p;
+  const void *src_a, *src_b;
+  void *pack_a, *pack_b;
+  float *db, *db_slab;
+  long long src_lda, src_ldb;
+  int a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, vec_a, vec_b, db_splits, epi, tile, f32;
 };
 
 enum : int { EPI_FPROP = 0, EPI_DGRAD = 1, EPI_WGRAD = 2 };
@@ -118,24 +129,26 @@ __device__ __forceinline__ void lin_by_kind(const LinParams& p, F f) {
 }
 
 // ---- operand tiles in LDS ------------------------------------------------------------------------------------------------
-// A K step is 64 elements.  An operand tile of R rows (i or j) holds R x 64 bf16 in one of two layouts, both
-// written by the LDS DMA in pieces of 1 KiB (64 lanes x 16 bytes), the swizzle applied to the SOURCE address:
-//  k contiguous:   [R][64], 16-byte chunk c of row r at c ^ s(r): 16 rows x one chunk fall on 16 different bank groups.  A
+// A K step is BK = 64 elements of one part, or 32 elements of all three parts of an fp32 operand.  A tile of R rows (i or j)
+// holds R x BK bf16 in one of two layouts, both written by the LDS DMA in pieces of 1 KiB (64 lanes x 16 bytes), the swizzle
+// applied to the SOURCE address:
+//  k contiguous:   [R][BK], 16-byte chunk c of row r at c ^ s(r): 16 rows x one chunk fall on 16 different bank groups.  A
 //                  fragment (lane l: row l & 15, 8 elements from k = 8 (l >> 4)) is one ds_read_b128.
-//  k strided (T):  [64][R], rows of R elements; a unit of 16 elements (32 bytes) u of row k at u ^ g(k).  A fragment is two
+//  k strided (T):  [BK][R], rows of R elements; a unit of 16 elements (32 bytes) u of row k at u ^ g(k).  A fragment is two
 //                  ds_read_b64_tr_b16: 16 lanes read 4 rows x 16 elements and get them transposed.  g spreads the 8 rows that
 //                  32 lanes read over the 64 banks.
 template <int R> __device__ __forceinline__ int lin_g(int k) {
   return R >= 128 ? (k & 3) | (((k >> 3) & 1) << 2) : ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
 }
-__device__ __forceinline__ int lin_s(int r) { return (r >> 1) & 7; }
+template <int BK> __device__ __forceinline__ int lin_s(int r) { return BK == 64 ? (r >> 1) & 7 : -(r >> 2) & 3; }
 
 // source of one 16-byte chunk of a piece in this lane at K step 0 of part 0; k: the chunk's first k in the step
-template <int R, bool T>
+template <int R, bool T, int BK>
 __device__ __forceinline__ const bf16_t* lin_source(const void* base, long long ld, int r0, int limit, int piece, int lane, int& k) {
   if (!T) {
-    const int r = piece * 8 + (lane >> 3);
-    k = ((lane & 7) ^ lin_s(r)) * 8;
+    constexpr int CPR = BK / 8;                          // chunks in a row
+    const int r = piece * (64 / CPR) + lane / CPR;
+    k = ((lane % CPR) ^ lin_s<BK>(r)) * 8;
     return (const bf16_t*)base + (long long)min(r0 + r, limit - 1) * ld + k;
   }
   constexpr int KPP = 512 / R, LPR = R / 8;              // rows of k in a piece, lanes per row
@@ -145,10 +158,10 @@ __device__ __forceinline__ const bf16_t* lin_source(const void* base, long long 
 }
 
 // One 16-row fragment of K part ks (32 elements).
-template <int R, bool T>
+template <int R, bool T, int BK>
 __device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int lane) {
   const int l15 = lane & 15, q4 = lane >> 4;
-  if (!T) return *(const bf16x8*)(t + (u * 16 + l15) * 128 + ((ks * 4 + q4) ^ lin_s(l15)) * 16);
+  if (!T) return *(const bf16x8*)(t + (u * 16 + l15) * (BK * 2) + ((ks * 4 + q4) ^ lin_s<BK>(l15)) * 16);
   const int k = ks * 32 + q4 * 8 + (l15 >> 2);
   const char* a = t + k * (R * 2) + (u ^ lin_g<R>(k)) * 32 + (l15 & 3) * 8;
   const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) bf16x4*)a);
@@ -156,26 +169,29 @@ __device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// this wave's pieces have landed and its LDS reads are done; behind the barrier, everyone's
-__device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// all but this wave's newest N pieces have landed and its LDS reads are done; behind the barrier, everyone's
+template <int N> __device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// The blocks are persistent and see ONE stream of K steps across their tiles: while step s is multiplied, step s + 1 lands, and
-// step s + 2 is requested as soon as the buffer of step s is free, also when it belongs to the next tile, so the epilogue of
-// a tile runs under the first loads of the next.  A step has four phases, each the matrix instructions of half the wave's
-// rows and half the step; a phase first reads the fragments of the NEXT phase from LDS.  The barrier stands before the last
-// phase: behind it everyone's reads of the buffer are done (registers hold what is left to multiply) and everyone's pieces
-// of step s + 1 have landed.
-template <typename T, int WM, int WN, int MT, int NT, int EPI>
-__global__ void __launch_bounds__(WM * WN * 64, 2) lin_mfma_kernel(LinParams p) {
+// The blocks are persistent and see ONE stream of K steps across their tiles, S of them in LDS: while step s is multiplied, the
+// steps behind it land, and step s + S is requested as soon as the buffer of step s is free, also when it belongs to the next
+// tile, so the epilogue of a tile runs under the first loads of the next.
+// P = 1: a step has four phases, each the matrix instructions of half the wave's rows and half the step; a phase first reads
+// the fragments of the NEXT phase from LDS.  The barrier stands before the last phase: behind it everyone's reads of the
+// buffer are done (registers hold what is left to multiply) and everyone's pieces of step s + 1 have landed.
+// P = 3: all three parts of both operands, each fragment read once for the six products of fp32 (P = 1 on parts walks over
+// them six times).  Half the LDS and DMA traffic, for tiles of which a CU has no second one to hide it behind; the larger
+// tile has no registers for it.  The fragments of step s + 1 are read while step s is multiplied.
+template <typename T, int WM, int WN, int MT, int NT, int S, int P, int EPI>
+__global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mfma_kernel(LinParams p) {
   constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
-  constexpr int BM = WM * MT * 16, BN = WN * NT * 16, NW = WM * WN, H = MT / 2;
-  constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
-  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // 1 KiB pieces a wave stages per step
-  static_assert(PA >= 1 && PB >= 1 && MT % 2 == 0 && MT <= 8 && NT % 2 == 0, "tile");
+  constexpr int BM = WM * MT * 16, BN = WN * NT * 16, NW = WM * WN, H = MT / 2, BK = P == 1 ? 64 : 32;
+  constexpr int A_PART = BM * BK * 2, B_PART = BN * BK * 2, A_BYTES = P * A_PART, STAGE = A_BYTES + P * B_PART;
+  constexpr int PA = A_BYTES / 1024 / NW, PB = (STAGE - A_BYTES) / 1024 / NW, PP = PA + PB;      // 1 KiB pieces a wave stages per step
+  static_assert(PA >= 1 && PB >= 1 && MT % 2 == 0 && MT <= 8 && NT % 2 == 0 && S >= 2 && S <= 4, "tile");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int tm = (p.rows + BM - 1) / BM, tn = (p.cols + BN - 1) / BN, tiles = tm * tn, jobs = tiles * p.splits;
-  const int ksteps = (p.K + 63) / 64, total = ksteps * (p.parts == 1 ? 1 : 6), per = (total + p.splits - 1) / p.splits;
+  const int ksteps = (p.K + BK - 1) / BK, passes = P == 1 && p.parts == 3 ? 6 : 1, total = ksteps * passes, per = (total + p.splits - 1) / p.splits;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
 
   // blocks of one XCD get neighbouring tiles: panels of 8 tile rows, walked column by column
@@ -189,91 +205,151 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) lin_mfma_kernel(LinParams p) 
   // ---- the stream of requests
   const bf16_t* ap[PA]; const bf16_t* bp[PB];
   int ak[PA], bk[PB];
-  int d_job = blockIdx.x, d_kt = 0, d_end = 0;
+  int d_job = blockIdx.x, d_kt = 0, d_end = 0, d_buf = 0;
   auto d_place = [&]() {
     int i0, j0, split;
     place(d_job, i0, j0, split);
     d_kt = split * per; d_end = min(d_kt + per, total);
+    auto part = [](const bf16_t* at, int part, long long stride) { return P == 1 ? at : at + part * stride; };
 #pragma unroll
-    for (int q = 0; q < PA; ++q) ap[q] = lin_source<BM, AT>(p.a, p.lda, i0, p.rows, wave * PA + q, lane, ak[q]);
-#pragma unroll
-    for (int q = 0; q < PB; ++q) bp[q] = lin_source<BN, BT>(p.b, p.ldb, j0, p.cols, wave * PB + q, lane, bk[q]);
-  };
-  auto request = [&](int to) __attribute__((always_inline)) {
-    if (d_job >= jobs) return;
-    const int seg = p.parts == 1 ? 0 : d_kt / ksteps, ks = d_kt - seg * ksteps;
-    // parts of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-    const int pa = p.parts == 1 ? 0 : (0x001102 >> (seg * 4)) & 15, pb = p.parts == 1 ? 0 : (0x010120 >> (seg * 4)) & 15;
-    const long long oa = pa * p.a_part + (AT ? ks * 64 * p.lda : (long long)ks * 64);
-    const long long ob = pb * p.b_part + (BT ? ks * 64 * p.ldb : (long long)ks * 64);
-    const int left = p.K - ks * 64;
-    const uint32_t stage = lds0 + to * STAGE;
-    if (left < 64) {          // the last step of an odd reduction: zeros behind its end
-#pragma unroll
-      for (int q = 0; q < PA; ++q) dpa_glds16(ak[q] < left ? ap[q] + oa : (const bf16_t*)lin_zero, stage + (wave * PA + q) * 1024);
-#pragma unroll
-      for (int q = 0; q < PB; ++q) dpa_glds16(bk[q] < left ? bp[q] + ob : (const bf16_t*)lin_zero, stage + A_BYTES + (wave * PB + q) * 1024);
-    } else {
-#pragma unroll
-      for (int q = 0; q < PA; ++q) dpa_glds16(ap[q] + oa, stage + (wave * PA + q) * 1024);
-#pragma unroll
-      for (int q = 0; q < PB; ++q) dpa_glds16(bp[q] + ob, stage + A_BYTES + (wave * PB + q) * 1024);
+    for (int q = 0; q < PA; ++q) {
+      const int piece = wave * PA + q, of = P == 1 ? 0 : piece / (A_PART / 1024);
+      ap[q] = part(lin_source<BM, AT, BK>(p.a, p.lda, i0, p.rows, piece - of * (A_PART / 1024), lane, ak[q]), of, p.a_part);
     }
-    if (++d_kt == d_end) { d_job += gridDim.x; if (d_job < jobs) d_place(); }
+#pragma unroll
+    for (int q = 0; q < PB; ++q) {
+      const int piece = wave * PB + q, of = P == 1 ? 0 : piece / (B_PART / 1024);
+      bp[q] = part(lin_source<BN, BT, BK>(p.b, p.ldb, j0, p.cols, piece - of * (B_PART / 1024), lane, bk[q]), of, p.b_part);
+    }
+  };
+  // A request is made piece by piece between matrix instructions: a block of them holds the wave until the address unit has
+  // taken each (16 cycles a piece for every wave of the CU), and the matrix pipe idles behind it.  Behind the last step the
+  // stream goes on with the last one again, into buffers that nobody reads any more.
+  long long oa = 0, ob = 0;
+  int left = 0;
+  uint32_t stage = 0;
+  auto next_step = [&]() __attribute__((always_inline)) {
+    const int pass = passes == 1 ? 0 : d_kt / ksteps, ks = d_kt - pass * ksteps;
+    // parts of the six products, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+    const int pa = passes == 1 ? 0 : (0x001102 >> (pass * 4)) & 15, pb = passes == 1 ? 0 : (0x010120 >> (pass * 4)) & 15;
+    oa = pa * p.a_part + (AT ? ks * BK * p.lda : (long long)ks * BK);
+    ob = pb * p.b_part + (BT ? ks * BK * p.ldb : (long long)ks * BK);
+    left = p.K - ks * BK;
+    stage = lds0 + d_buf * STAGE;
+    d_buf = d_buf + 1 == S ? 0 : d_buf + 1;
+  };
+  auto request = [&](int q) __attribute__((always_inline)) {          // (zeros behind the end of an odd reduction)
+    if (q < PA) dpa_glds16(ak[q] < left ? ap[q] + oa : (const bf16_t*)lin_zero, stage + (wave * PA + q) * 1024);
+    else dpa_glds16(bk[q - PA] < left ? bp[q - PA] + ob : (const bf16_t*)lin_zero, stage + A_BYTES + (wave * PB + q - PA) * 1024);
+  };
+  auto requested = [&]() __attribute__((always_inline)) {
+    if (++d_kt == d_end) { if (d_job + (int)gridDim.x < jobs) { d_job += gridDim.x; d_place(); } else --d_kt; }
   };
 
   f32x4 acc[MT][NT];
-  bf16x8 fa[MT], fb[2][NT];
-  auto read_a = [&](int buf, int half, int ks) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < H; ++i) fa[half * H + i] = lin_fragment<BM, AT>(smem + buf * STAGE, wm * MT + half * H + i, ks, lane);
+  // operands of the matrix instructions in (j, i) order: a lane then holds four neighbouring columns of one output row
+  auto mfma = [](bf16x8 b, bf16x8 a, f32x4& c) __attribute__((always_inline)) { c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0); };
+  auto a_at = [&](int buf, int part, int i, int ks) __attribute__((always_inline)) {
+    return lin_fragment<BM, AT, BK>(smem + buf * STAGE + part * A_PART, wm * MT + i, ks, lane);
   };
-  auto read_b = [&](int buf, int ks) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) fb[ks][j] = lin_fragment<BN, BT>(smem + buf * STAGE + A_BYTES, wn * NT + j, ks, lane);
-  };
-  auto multiply = [&](int half, int ks) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < H; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)          // (j rows, i columns: a lane then holds four neighbouring columns of one output row)
-        acc[half * H + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[ks][j], fa[half * H + i], acc[half * H + i][j], 0, 0, 0);
+  auto b_at = [&](int buf, int part, int j, int ks) __attribute__((always_inline)) {
+    return lin_fragment<BN, BT, BK>(smem + buf * STAGE + A_BYTES + part * B_PART, wn * NT + j, ks, lane);
   };
 
   d_place();
-  request(0);
-  request(1);
-  lin_sync();
+#pragma unroll 1
+  for (int k = 0; k < S; ++k) {
+    next_step();
+#pragma unroll
+    for (int q = 0; q < PP; ++q) request(q);
+    requested();
+  }
+  lin_sync<(S - 1) * PP>();
   int buf = 0;
   for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
     int i0, j0, split;
     place(job, i0, j0, split);
-    const int kt0 = split * per, kt1 = min(kt0 + per, total);
-    read_b(buf, 0);
-    read_a(buf, 0, 0);
+    int steps = min((split + 1) * per, total) - split * per;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int kt = kt0; kt < kt1; ++kt) {
-      read_a(buf, 1, 0);
-      multiply(0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      read_b(buf, 1);
-      read_a(buf, 0, 1);
-      multiply(1, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      read_a(buf, 1, 1);
-      multiply(0, 1);
-      lin_sync();
-      request(buf);
-      buf ^= 1;
-      if (kt + 1 < kt1) {
-        read_b(buf, 0);
-        read_a(buf, 0, 0);
+    if constexpr (P == 1) {
+      bf16x8 fa[MT], fb[2][NT];
+      auto read_a = [&](int half, int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) fa[half * H + i] = a_at(buf, 0, half * H + i, ks);
+      };
+      auto read_b = [&](int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[ks][j] = b_at(buf, 0, j, ks);
+      };
+      auto multiply = [&](int half, int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mfma(fb[ks][j], fa[half * H + i], acc[half * H + i][j]);
+      };
+      read_b(0);
+      read_a(0, 0);
+      for (; steps > 0; --steps) {
+        read_a(1, 0);
+        multiply(0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        read_b(1);
+        read_a(0, 1);
+        multiply(1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        read_a(1, 1);
+        multiply(0, 1);
+        lin_sync<(S - 2) * PP>();
+        buf = buf + 1 == S ? 0 : buf + 1;
+        if (steps > 1) {
+          read_b(0);
+          read_a(0, 0);
+        }
+        next_step();
+#pragma unroll
+        for (int n = 0; n < H * NT; ++n) {
+#pragma unroll
+          for (int q = n * PP / (H * NT); q < (n + 1) * PP / (H * NT); ++q) { request(q); __builtin_amdgcn_sched_barrier(0); }
+          mfma(fb[1][n % NT], fa[H + n / NT], acc[H + n / NT][n % NT]);
+        }
+        requested();
+        __builtin_amdgcn_sched_barrier(0);
       }
-      multiply(1, 1);
-      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      struct Parts { bf16x8 a[P][MT], b[P][NT]; } even, odd;
+      auto read = [&](Parts& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = P - 1; q >= 0; --q) {          // (in the order of use)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) f.a[q][i] = a_at(buf, q, i, 0);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) f.b[P - 1 - q][j] = b_at(buf, P - 1 - q, j, 0);
+        }
+      };
+      auto step = [&](Parts& f, Parts& next, bool more) __attribute__((always_inline)) {
+        lin_sync<(S - 2) * PP>();          // (this wave's reads of the step are done: its buffer is free behind the barrier)
+        buf = buf + 1 == S ? 0 : buf + 1;
+        if (more) read(next);
+        next_step();
+        constexpr int EACH = 6 * MT * NT / PP;
+#pragma unroll
+        for (int n = 0; n < 6 * MT * NT; ++n) {          // parts (a, b), smallest products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+          const int q = n / (MT * NT), i = n / NT % MT, j = n % NT;
+          if (n % EACH == 0 && n / EACH < PP) { request(n / EACH); __builtin_amdgcn_sched_barrier(0); }
+          mfma(f.b[(0x010120 >> (q * 4)) & 15][j], f.a[(0x001102 >> (q * 4)) & 15][i], acc[i][j]);
+        }
+        requested();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      read(even);
+      for (; steps > 1; steps -= 2) {
+        step(even, odd, true);
+        step(odd, even, steps > 2);
+      }
+      if (steps) step(even, odd, false);
     }
 
     // ---- epilogue, from registers.  Neighbouring 16-column tiles trade quarters, so that a lane holds 8 columns of one row,
@@ -351,6 +427,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) lin_mfma_kernel(LinParams p) 
       });
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // no piece is on its way to LDS that is no longer this block's
 }
 
 // joins the partial products of a split reduction in a fixed order and applies the epilogue
@@ -362,6 +439,7 @@ __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p) {
   for (long long t = blockIdx.x * 256LL + threadIdx.x; t < total; t += gridDim.x * 256LL) {
     const int i = (int)(t / groups), j = (int)(t - (long long)i * groups) * 8, n = min(8, p.cols - j);
     float v[8] = {};
+#pragma unroll 4
     for (int k = 0; k < p.splits; ++k) {
       Lin8<float> s;
       const float* w = p.ws + k * part + (long long)i * p.cols + j;
@@ -377,16 +455,25 @@ __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p) {
   }
 }
 
-template <typename T, int WM, int WN, int MT, int NT, int EPI>
+// Blocks on the chip at a time: a multiple of 8 where a launch has several rounds (xcd_remap).
+template <typename T, int WM, int WN, int MT, int NT, int S, int P, int EPI>
 static int lin_run(const LinParams& p, hipStream_t s) {
   constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
-  constexpr int lds = 2 * (BM + BN) * 128, residents = 160 * 1024 / lds;
+  constexpr int lds = S * (BM + BN) * (P == 1 ? 128 : 192), residents = 160 * 1024 / lds;
   const long long jobs = (long long)((p.rows + BM - 1) / BM) * ((p.cols + BN - 1) / BN) * p.splits;
   if (jobs > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
-  static const int once = (int)hipFuncSetAttribute((const void*)lin_mfma_kernel<T, WM, WN, MT, NT, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (once) return once;
-  const int grid = (int)(jobs < 256 * residents ? jobs : 256 * residents);      // (a multiple of 8 where there are several rounds: xcd_remap)
-  lin_mfma_kernel<T, WM, WN, MT, NT, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
+  if (lds > 64 * 1024) {          // once for each device; a lost race sets it twice
+    static std::atomic<unsigned> done[64];
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
+    if (dev >= 64 || !done[dev].load(std::memory_order_relaxed)) {
+      const hipError_t e = hipFuncSetAttribute((const void*)lin_mfma_kernel<T, WM, WN, MT, NT, S, P, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e) return (int)e;
+      if (dev < 64) done[dev].store(1, std::memory_order_relaxed);
+    }
+  }
+  const int grid = (int)(jobs < 256 * residents ? jobs : 256 * residents);
+  lin_mfma_kernel<T, WM, WN, MT, NT, S, P, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
   if (p.splits > 1) lin_join_kernel<T, EPI><<<dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256), 256, 0, s>>>(p);
   return dpa_launch_rc();
 }
@@ -394,9 +481,12 @@ static int lin_run(const LinParams& p, hipStream_t s) {
 template <typename T, int EPI>
 static int lin_tile(const LinParams& p, int tile, hipStream_t s) {
   switch (tile) {
-    case 0: return lin_run<T, 2, 4, 8, 4, EPI>(p, s);      // 256 x 256, 8 waves
-    case 1: return lin_run<T, 2, 2, 4, 4, EPI>(p, s);      // 128 x 128, 4 waves
-    case 2: return lin_run<T, 2, 2, 2, 2, EPI>(p, s);      // 64 x 64, 4 waves
+    case 0: return lin_run<T, 2, 4, 8, 4, 2, 1, EPI>(p, s);      // 256 x 256, 8 waves
+    case 1: return lin_run<T, 2, 2, 4, 4, 2, 1, EPI>(p, s);      // 128 x 128, 4 waves, two blocks a CU
+    case 2: return lin_run<T, 2, 2, 4, 4, 4, 1, EPI>(p, s);      // 128 x 128, four steps in LDS
+    case 3: return lin_run<T, 2, 2, 2, 2, 4, 1, EPI>(p, s);      // 64 x 64, two blocks a CU
+    case 4: if constexpr (sizeof(T) == 4) return lin_run<T, 2, 2, 4, 4, 3, 3, EPI>(p, s); break;      // 128 x 128, three parts at once
+    case 5: if constexpr (sizeof(T) == 4) return lin_run<T, 2, 2, 2, 2, 4, 3, EPI>(p, s); break;      // 64 x 64, three parts at once
   }
   return (int)hipErrorInvalidValue;
 }

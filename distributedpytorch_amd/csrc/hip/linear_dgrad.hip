@@ -2,5 +2,5 @@
 #include "linear.h"
 
 int lin_dgrad(const LinParams& p, int tile, hipStream_t s) {
-  return p.out32 ? lin_tile<float, EPI_DGRAD>(p, tile, s) : lin_tile<bf16_t, EPI_DGRAD>(p, tile, s);
+  return p.parts == 3 ? lin_tile<float, EPI_DGRAD>(p, tile, s) : lin_tile<bf16_t, EPI_DGRAD>(p, tile, s);
 }

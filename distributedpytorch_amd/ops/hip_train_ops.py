@@ -1,16 +1,20 @@
 """Group norm, linear products with epilogues and AdamW on the GPU: checks (ops/checks.py), workspaces and launches of
 csrc/hip/group_norm.hip, linear.hip and adamw.hip.  Workspaces are torch allocations of the call: they belong to its
-stream, and to its graph where the call is captured, so no two calls share one."""
+stream, and to its graph where the call is captured, so no two calls share one.
+
+A small call is bound by what the host does before the launch: everything here works on plain integers, and each operator
+is one call into the library."""
 from __future__ import annotations
 
 import ctypes
+from ctypes import byref
 
 import torch
 
-from . import checks, native, ref_ops
-from .native import I32, I64, VP, F32, _OnDevice, ptr
+from . import checks, native
+from .native import F32, I32, I64, VP
 
-_DT = {torch.float32: 0, torch.bfloat16: 1}
+_F32, _BF16 = torch.float32, torch.bfloat16
 
 
 class GnParams(ctypes.Structure):
@@ -20,23 +24,36 @@ class GnParams(ctypes.Structure):
                 ("N", I32), ("HW", I32), ("C", I32), ("G", I32), ("cg", I32), ("S", I32), ("pps", I32), ("eps", F32)]
 
 
-class LinParams(ctypes.Structure):
+class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
     _fields_ = [("a", VP), ("b", VP), ("lda", I64), ("ldb", I64), ("a_part", I64), ("b_part", I64), ("bias", VP), ("addend", VP), ("pre", VP),
                 ("out", VP), ("preact", VP), ("ws", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
-                ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("out32", I32),
-                ("vec", I32), ("bias_vec", I32)]
+                ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("vec", I32),
+                ("bias_vec", I32), ("pad", I32),
+                ("src_a", VP), ("src_b", VP), ("pack_a", VP), ("pack_b", VP), ("db", VP), ("db_slab", VP), ("src_lda", I64), ("src_ldb", I64),
+                ("a_rows", I32), ("a_cols", I32), ("b_rows", I32), ("b_cols", I32), ("ld_a", I32), ("ld_b", I32), ("vec_a", I32), ("vec_b", I32),
+                ("db_splits", I32), ("epi", I32), ("tile", I32), ("f32", I32)]
 
 
-_checked = []
+_loaded = []
 
 
 def _lib():
+    if _loaded:
+        return _loaded[0]
     lib = native.hip_lib()
-    if not _checked:
-        if lib.dpa_gn_params_size() != ctypes.sizeof(GnParams) or lib.dpa_lin_params_size() != ctypes.sizeof(LinParams):
-            raise RuntimeError("GnParams / LinParams ABI mismatch between ops/hip_train_ops.py and csrc/hip")
-        _checked.append(True)
+    if lib.dpa_gn_params_size() != ctypes.sizeof(GnParams) or lib.dpa_lin_params_size() != ctypes.sizeof(LinCall):
+        raise RuntimeError("GnParams / LinCall ABI mismatch between ops/hip_train_ops.py and csrc/hip")
+    _loaded.append(lib)
     return lib
+
+
+def _run(device, body, *args):
+    """body(stream, *args) with the tensors' device as the current one, on its current stream"""
+    i = device.index
+    if i == torch._C._cuda_getDevice():
+        return body(VP(torch._C._cuda_getCurrentRawStream(i)), *args)
+    with torch.cuda.device(device):
+        return body(VP(torch._C._cuda_getCurrentRawStream(i)), *args)
 
 
 # ----------------------------------------------------------------------------------------- group norm
@@ -48,172 +65,198 @@ def _gn_splits(n, hw, c):
     return (hw + pps - 1) // pps, pps
 
 
-def _gn_params(x, gamma, beta, groups, mean, rstd):
+def _gn_params(x, groups, vecs):
     n, h, w, c = x.shape
     p = GnParams()
-    p.x, p.gamma, p.beta, p.mean, p.rstd = ptr(x), ptr(gamma), ptr(beta), ptr(mean), ptr(rstd)
+    p.gamma, p.beta, p.mean, p.rstd = vecs[:4]
     p.N, p.HW, p.C, p.G, p.cg = n, h * w, c, groups, c // groups
     p.S, p.pps = _gn_splits(n, h * w, c)
     return p
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", residual=None):
-    cs = checks.group_norm("group_norm_fwd", x, gamma, beta, groups, mean, rstd)
-    a = checks.act_id(act)
-    y_cs = checks.nhwc(y, "group_norm_fwd: y", x.shape, x.dtype)
-    res_cs = 0 if residual is None else checks.nhwc(residual, "group_norm_fwd: residual", x.shape, x.dtype)
-    checks.same_device("group_norm_fwd", x, y=y, residual=residual)
-    checks.overlap("group_norm_fwd", y, x=x, residual=residual)
+    a, xs, ys, rs, vecs = checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
     if x.numel() == 0:
         return y
-    p = _gn_params(x, gamma, beta, groups, mean, rstd)
-    p.y, p.res, p.x_cs, p.y_cs, p.res_cs, p.eps = ptr(y), ptr(residual), cs, y_cs, res_cs, eps
-    with _OnDevice(x) as stream:
-        slab = torch.empty(p.N * p.S * 2 * p.C, device=x.device, dtype=torch.float32)
-        p.slab = ptr(slab)
-        _lib().dpa_group_norm_fwd(ctypes.byref(p), a, _DT[x.dtype], stream)
+    p = _gn_params(x, groups, vecs)
+    p.x, p.x_cs, _ = xs
+    p.y, p.y_cs, _ = ys
+    p.res, p.res_cs, _ = rs
+    p.eps = eps
+    _run(x.device, _gn_launch, p, x, p.N * p.S * 2 * p.C, _lib().dpa_group_norm_fwd, a)
     return y
 
 
 def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbeta=None, act="none", y=None, residual=None,
                    dresidual=None):
-    strides = ref_ops.check_group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
+    a, xs, dys, dxs, ys, rs, drs, vecs = checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y,
+                                                               residual, dresidual)
     if x.numel() == 0:
         for t in (dgamma, dbeta):
             if t is not None:
                 t.zero_()
         return dx
-    p = _gn_params(x, gamma, beta, groups, mean, rstd)
-    p.dy, p.dx, p.yv, p.res, p.dres = ptr(dy), ptr(dx), ptr(y), ptr(residual), ptr(dresidual)
-    p.x_cs, p.dy_cs, p.dx_cs, p.yv_cs, p.res_cs, p.dres_cs = strides
-    p.dgamma, p.dbeta = ptr(dgamma), ptr(dbeta)
-    with _OnDevice(x) as stream:
-        ws = torch.empty(p.N * p.S * 2 * p.C + 2 * p.N * p.G, device=x.device, dtype=torch.float32)
-        p.slab, p.coef = ptr(ws), VP(ws.data_ptr() + 4 * p.N * p.S * 2 * p.C)
-        _lib().dpa_group_norm_bwd(ctypes.byref(p), checks.act_id(act), _DT[x.dtype], stream)
+    p = _gn_params(x, groups, vecs)
+    p.dgamma, p.dbeta = vecs[4:]
+    p.x, p.x_cs, _ = xs
+    p.dy, p.dy_cs, _ = dys
+    p.dx, p.dx_cs, _ = dxs
+    p.yv, p.yv_cs, _ = ys
+    p.res, p.res_cs, _ = rs
+    p.dres, p.dres_cs, _ = drs
+    _run(x.device, _gn_launch, p, x, p.N * p.S * 2 * p.C, _lib().dpa_group_norm_bwd, a)
     return dx
 
 
+def _gn_launch(stream, p, x, slab, entry, act):
+    ws = torch.empty(slab + 2 * p.N * p.G, device=x.device, dtype=_F32)
+    p.slab = ws.data_ptr()
+    p.coef = p.slab + 4 * slab
+    entry(byref(p), act, int(x.dtype is _BF16), stream)
+
+
 # ----------------------------------------------------------------------------------------- linear products
-_FPROP, _DGRAD, _WGRAD = 0, 1, 2          # csrc/hip/linear.hip
-_TILES = ((256, 256), (128, 128), (64, 64))
+_FPROP, _DGRAD, _WGRAD = 0, 1, 2          # csrc/hip/linear.h
 
 
-def _plan(rows, cols, ksteps):
-    """(tile, splits of the reduction)"""
-    for i, (bm, bn) in enumerate(_TILES):
-        blocks = ((rows + bm - 1) // bm) * ((cols + bn - 1) // bn)
-        if blocks >= 200:
-            return i, 1
-    blocks = ((rows + 63) // 64) * ((cols + 63) // 64)
-    return 2, max(1, min(256 // blocks, ksteps // 4, 16))
+def _cdiv(a, b):
+    return (a + b - 1) // b
 
 
-def _aligned(t, ld):
-    es = t.element_size()
-    return t.data_ptr() % 16 == 0 and (ld * es) % 16 == 0
+def _plan(rows, cols, k, f32):
+    """(tile of lin_tile, splits of the reduction)"""
+    if _cdiv(rows, 256) * _cdiv(cols, 256) >= 200:
+        return 0, 1
+    t128 = _cdiv(rows, 128) * _cdiv(cols, 128)
+    if t128 >= 200:
+        return (4 if f32 else 1 if t128 > 256 else 2), 1
+    t64 = _cdiv(rows, 64) * _cdiv(cols, 64)
+    return (5 if f32 else 3), max(1, min(512 // t64, k // 256, 16))
 
 
-def _operand(t, ld, stream, keep):
-    """(pointer, row stride, stride of its parts, parts): the matrix as the kernel's DMA takes it - bf16 rows of a multiple
-    of 8 elements at 16-byte addresses as they are, anything else through lin_pack_kernel."""
-    rows, cols = t.shape
-    f32 = t.dtype == torch.float32
-    if not f32 and cols % 8 == 0 and _aligned(t, ld):
-        return ptr(t), ld, 0
-    ldd = (cols + 7) // 8 * 8
-    buf = torch.empty((3 if f32 else 1) * rows * ldd, device=t.device, dtype=torch.bfloat16)
-    keep.append(buf)
-    if rows:
-        _lib().dpa_linear_pack(ptr(t), I64(ld), rows, cols, ldd, int(_aligned(t, ld)), ptr(buf), _DT[t.dtype], stream)
-    return ptr(buf), ldd, rows * ldd
-
-
-def _product(epi, a, lda, b, ldb, p, k, stream, keep):
-    p.a, p.lda, p.a_part = _operand(a, lda, stream, keep)
-    p.b, p.ldb, p.b_part = _operand(b, ldb, stream, keep)
-    p.K, p.parts = k, 3 if a.dtype == torch.float32 else 1
-    tile, p.splits = _plan(p.rows, p.cols, (k + 63) // 64 * (6 if p.parts == 3 else 1))
-    if p.splits > 1:
-        ws = torch.empty(p.splits * p.rows * p.cols, device=a.device, dtype=torch.float32)
-        keep.append(ws)
-        p.ws = ptr(ws)
-    _lib().dpa_linear(ctypes.byref(p), epi, tile, stream)
-
-
-def _vec(cols, *mats):
-    return int(cols % 8 == 0 and all(t is None or _aligned(t, ld) for t, ld in mats))
+def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
+    """Fills in the operands, the plan and the workspace of a call whose epilogue is set, and launches it."""
+    c.src_a, c.src_lda, _ = a
+    c.src_b, c.src_ldb, _ = b
+    c.a_rows, c.a_cols = t_a.shape
+    c.b_rows, c.b_cols = t_b.shape
+    f32 = c.f32
+    es = 4 if f32 else 2
+    c.vec_a = ok_a = not (a[0] | a[1] * es) & 15
+    c.vec_b = ok_b = not (b[0] | b[1] * es) & 15
+    c.K, c.parts = k, 3 if f32 else 1
+    few = c.epi == _FPROP and c.rows <= 64 and ok_a and ok_b and not (k * es) & 15
+    c.a, c.lda, c.b, c.ldb = a[0], a[1], b[0], b[1]
+    need = 0
+    if few:
+        c.tile, c.splits = -1, 1
+    else:
+        c.tile, c.splits = _plan(c.rows, c.cols, k, f32)
+        # the DMA takes bf16 rows of a multiple of 8 elements at 16-byte addresses as they are; anything else is packed
+        if f32 or not ok_a or c.a_cols & 7:
+            c.ld_a = c.lda = (c.a_cols + 7) & ~7
+            c.a_part = c.a_rows * c.lda
+            need += c.parts * c.a_part * 2 + 15 & ~15
+        if f32 or not ok_b or c.b_cols & 7:
+            c.ld_b = c.ldb = (c.b_cols + 7) & ~7
+            c.b_part = c.b_rows * c.ldb
+            need += c.parts * c.b_part * 2 + 15 & ~15
+        if c.splits > 1:
+            steps = _cdiv(k, 32 if c.tile >= 4 else 64) * (6 if f32 and c.tile < 4 else 1)
+            c.splits = _cdiv(steps, _cdiv(steps, c.splits))          # no range is empty
+            need += c.splits * c.rows * c.cols * 4 + 15 & ~15
+    need += db_slab * 4
+    if need:
+        ws = torch.empty(need, device=device, dtype=torch.uint8)
+        at = ws.data_ptr()
+        if c.ld_a:
+            c.a = c.pack_a = at
+            at += c.parts * c.a_part * 2 + 15 & ~15
+        if c.ld_b:
+            c.b = c.pack_b = at
+            at += c.parts * c.b_part * 2 + 15 & ~15
+        if c.splits > 1:
+            c.ws = at
+            at += c.splits * c.rows * c.cols * 4 + 15 & ~15
+        c.db_slab = at
+    _lib().dpa_linear(byref(c), stream)
 
 
 def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
-    ldx, ldw, ldy, lda, ldz = ref_ops.check_linear_fprop(x, w, y, bias, act, addend, preact)
-    if x.shape[0] == 0:
+    a, xs, ws, ys, ads, zs, b = checks.linear_fprop(x, w, y, bias, act, addend, preact)
+    m, k = x.shape
+    if m == 0:
         return y
-    p = LinParams()
-    p.bias, p.addend, p.out, p.preact = ptr(bias), ptr(addend), ptr(y), ptr(preact)
-    p.ld_add, p.ld_out, p.ld_z = lda, ldy, ldz
-    p.rows, p.cols, p.act, p.out32 = x.shape[0], w.shape[0], checks.act_id(act), int(x.dtype == torch.float32)
-    p.vec = _vec(p.cols, (y, ldy), (addend, lda), (preact, ldz))
-    p.bias_vec = int(bias is not None and p.cols % 8 == 0 and bias.data_ptr() % 16 == 0)
-    keep = []
-    with _OnDevice(x) as stream:
-        _product(_FPROP, x, ldx, w, ldw, p, x.shape[1], stream, keep)
+    c = LinCall()
+    n = w.shape[0]
+    c.epi, c.rows, c.cols, c.act, c.bias = _FPROP, m, n, a, b
+    c.out, c.ld_out, _ = ys
+    c.addend, c.ld_add, _ = ads
+    c.preact, c.ld_z, _ = zs
+    f32 = c.f32 = x.dtype is _F32
+    c.vec = not (n & 7 or (ys[0] | ads[0] | zs[0] | (ys[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
+    c.bias_vec = not (n & 7 or b & 15)
+    _run(x.device, _linear, c, x, xs, w, ws, k, x.device, 0)
     return y
 
 
 def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
-    ldy, ldw, ldx, ldp, lda = ref_ops.check_linear_dgrad(dy, w, dx, act, preact, addend)
-    if dy.shape[0] == 0:
+    a, dys, ws, dxs, zs, ads = checks.linear_dgrad(dy, w, dx, act, preact, addend)
+    m, n = dy.shape
+    if m == 0:
         return dx
-    p = LinParams()
-    p.addend, p.pre, p.out = ptr(addend), ptr(preact), ptr(dx)
-    p.ld_add, p.ld_pre, p.ld_out = lda, ldp, ldx
-    p.rows, p.cols, p.act, p.out32 = dy.shape[0], w.shape[1], checks.act_id(act), int(dy.dtype == torch.float32)
-    p.vec = _vec(p.cols, (dx, ldx), (addend, lda), (preact, ldp))
-    keep = []
-    with _OnDevice(dy) as stream:
-        _product(_DGRAD, dy, ldy, w, ldw, p, dy.shape[1], stream, keep)
+    c = LinCall()
+    k = w.shape[1]
+    c.epi, c.rows, c.cols, c.act = _DGRAD, m, k, a
+    c.out, c.ld_out, _ = dxs
+    c.pre, c.ld_pre, _ = zs
+    c.addend, c.ld_add, _ = ads
+    f32 = c.f32 = dy.dtype is _F32
+    c.vec = not (k & 7 or (dxs[0] | ads[0] | zs[0] | (dxs[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
+    _run(dy.device, _linear, c, dy, dys, w, ws, n, dy.device, 0)
     return dx
 
 
 def linear_wgrad(dy, x, dw, db=None, accumulate=False):
-    ldy, ldx, ldw = ref_ops.check_linear_wgrad(dy, x, dw, db)
-    p = LinParams()
-    p.out, p.ld_out, p.accumulate = ptr(dw), ldw, int(accumulate)
-    p.rows, p.cols = dy.shape[1], x.shape[1]
-    p.vec = _vec(p.cols, (dw, ldw))
-    keep = []
-    with _OnDevice(dy) as stream:
-        _product(_WGRAD, dy, ldy, x, ldx, p, dy.shape[0], stream, keep)
-        if db is not None:
-            m, n = dy.shape
-            splits = max(1, min((m + 63) // 64, 2048 // ((n + 63) // 64), 64))
-            per = max(1, (m + splits - 1) // splits)
-            slab = torch.empty(splits * n, device=dy.device, dtype=torch.float32)
-            _lib().dpa_linear_colsum(ptr(dy), I64(ldy), m, n, splits, per, ptr(slab), int(accumulate), ptr(db), _DT[dy.dtype], stream)
+    dys, xs, dws, b = checks.linear_wgrad(dy, x, dw, db)
+    m, n = dy.shape
+    if m == 0:
+        if not accumulate:
+            dw.zero_()
+            if db is not None:
+                db.zero_()
+        return dw
+    c = LinCall()
+    k = x.shape[1]
+    c.epi, c.rows, c.cols, c.accumulate, c.db = _WGRAD, n, k, int(accumulate), b
+    c.out, c.ld_out, _ = dws
+    c.f32 = dy.dtype is _F32
+    c.vec = not (k & 7 or (dws[0] | dws[1] * 4) & 15)
+    slab = 0
+    if b:
+        c.db_splits = max(1, min(_cdiv(m, 32), 1024 // _cdiv(n, 512)))
+        slab = c.db_splits * n
+    _run(dy.device, _linear, c, dy, dys, x, xs, m, dy.device, slab)
     return dw
 
 
 # ----------------------------------------------------------------------------------------- AdamW
-def _at(t, lo, esize):
-    return VP(t.data_ptr() + lo * esize) if t is not None else VP(0)
-
-
 def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
     n = p.numel()
-    hi = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi,
-                      {"m": (m, torch.float32, n), "v": (v, torch.float32, n)})
-    with _OnDevice(p) as stream:
-        _lib().dpa_adamw_step(_at(p, lo, 4), _at(g, lo, 4), _at(m, lo, 4), _at(v, lo, 4), _at(p16, lo, 2), ptr(hyper), ptr(groups),
-                              _at(group_ids, lo // 64, 1), I64(hi - lo), stream)
+    hi, at = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi, (("m", m, _F32, n), ("v", v, _F32, n)))
+    ap, ag, a16, ah, agr, aid, am, av = at
+    b = 4 * lo
+    _run(p.device, lambda stream: _lib().dpa_adamw_step(VP(ap + b), VP(ag + b), VP(am + b), VP(av + b), VP(a16 and a16 + 2 * lo), VP(ah), VP(agr),
+                                                        VP(aid + lo // 64), I64(hi - lo), stream))
 
 
 def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, seed, lo=0, hi=None):
     n = p.numel()
-    hi = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
-                      {"m": (m, torch.float8_e4m3fn, n), "v": (v, torch.float8_e5m2, n),
-                       "m_scale": (m_scale, torch.float32, n // 64), "v_scale": (v_scale, torch.float32, n // 64)})
-    with _OnDevice(p) as stream:
-        _lib().dpa_adamw8_step(_at(p, lo, 4), _at(g, lo, 4), _at(m, lo, 1), _at(v, lo, 1), _at(m_scale, lo // 64, 4),
-                               _at(v_scale, lo // 64, 4), _at(p16, lo, 2), ptr(hyper), ptr(groups), _at(group_ids, lo // 64, 1),
-                               ctypes.c_uint(seed & 0xFFFFFFFF), I64(lo), I64(hi - lo), stream)
+    hi, at = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
+                          (("m", m, torch.float8_e4m3fn, n), ("v", v, torch.float8_e5m2, n), ("m_scale", m_scale, _F32, n // 64),
+                           ("v_scale", v_scale, _F32, n // 64)))
+    ap, ag, a16, ah, agr, aid, am, av, ams, avs = at
+    b, s = 4 * lo, lo // 16
+    _run(p.device, lambda stream: _lib().dpa_adamw8_step(VP(ap + b), VP(ag + b), VP(am + lo), VP(av + lo), VP(ams + s), VP(avs + s),
+                                                         VP(a16 and a16 + 2 * lo), VP(ah), VP(agr), VP(aid + lo // 64),
+                                                         ctypes.c_uint(seed & 0xFFFFFFFF), I64(lo), I64(hi - lo), stream))

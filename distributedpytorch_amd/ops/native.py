@@ -74,22 +74,6 @@ class KernelLaunchError(RuntimeError):
     pass
 
 
-class _OnDevice:
-    """Launches go to the tensors' device and its current stream, also while another device is the current one."""
-
-    def __init__(self, t):
-        self._guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return stream_ptr()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
 class _CheckedLib:
     """The kernel library with every launching entry point's status checked: each DPA_API launcher returns
     hipGetLastError() (csrc/hip/common.h: dpa_launch_rc), and a rejected launch - too much dynamic LDS, an oversize

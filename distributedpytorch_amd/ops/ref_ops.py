@@ -536,13 +536,7 @@ def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", resid
     (fp32 [N, groups]) for the backward pass.  gamma, beta: fp32 [C].  act: "none", "relu", "silu" or "gelu".  y may be x
     or residual itself."""
     from . import checks
-    checks.group_norm("group_norm_fwd", x, gamma, beta, groups, mean, rstd)
-    checks.act_id(act)
-    checks.nhwc(y, "group_norm_fwd: y", x.shape, x.dtype)
-    if residual is not None:
-        checks.nhwc(residual, "group_norm_fwd: residual", x.shape, x.dtype)
-    checks.same_device("group_norm_fwd", x, y=y, residual=residual)
-    checks.overlap("group_norm_fwd", y, x=x, residual=residual)
+    checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
     if x.numel() == 0:
         return y
     t = _grouped(x.float(), groups)
@@ -564,7 +558,7 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
     None).  The activation's derivative is taken at values recomputed from x (and residual); for "relu" the stored output
     may be given as y instead, its sign is then the mask.  dx may be dy or x itself, dresidual may be dy, y or residual."""
     from . import checks
-    check_group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
+    checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
     if x.numel() == 0:
         for t in (dgamma, dbeta):
             if t is not None:
@@ -593,115 +587,13 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
     return dx
 
 
-def check_group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual):
-    """Channel strides (x, dy, dx, y, residual, dresidual), 0 for what is absent."""
-    from . import checks
-    name = "group_norm_bwd"
-    cs = [checks.group_norm(name, x, gamma, beta, groups, mean, rstd)]
-    checks.act_id(act)
-    for k, t in (("dy", dy), ("dx", dx), ("y", y), ("residual", residual), ("dresidual", dresidual)):
-        cs.append(0 if t is None else checks.nhwc(t, f"{name}: {k}", x.shape, x.dtype))
-    if y is not None and act != "relu":
-        raise ValueError(f"{name}: y is the mask of a ReLU; act is {act!r}")
-    for k, t in (("dgamma", dgamma), ("dbeta", dbeta)):
-        if t is not None:
-            checks.vec32(t, f"{name}: {k}", x.shape[3])
-    checks.same_device(name, x, dy=dy, dx=dx, y=y, residual=residual, dresidual=dresidual, dgamma=dgamma, dbeta=dbeta)
-    checks.overlap(name, dx, dy=dy, x=x, y=y, residual=residual)
-    if dresidual is not None:
-        checks.overlap(name, dresidual, dy=dy, y=y, residual=residual)
-        for k, t in (("x", x), ("dx", dx)):          # x is read again after dresidual was written
-            if dresidual.data_ptr() == t.data_ptr() and x.numel():
-                raise ValueError(f"{name}: dresidual may not be {k}")
-        checks.overlap(name, dresidual, x=x, dx=dx)
-    return cs
-
-
 # ----------------------------------------------------------------------------------------- linear products
-def check_linear_fprop(x, w, y, bias, act, addend, preact):
-    """Row strides (x, w, y, addend, preact)."""
-    from . import checks
-    name = "linear_fprop"
-    if x.dtype not in checks.FLOATS:
-        raise ValueError(f"{name}: x must be fp32 or bf16, got {x.dtype}")
-    ld = [checks.mat(x, f"{name}: x"), checks.mat(w, f"{name}: w", None, x.shape[1], x.dtype)]
-    m, n = x.shape[0], w.shape[0]
-    checks.act_id(act)
-    for k, t in (("y", y), ("addend", addend), ("preact", preact)):
-        ld.append(0 if t is None else checks.mat(t, f"{name}: {k}", m, n, x.dtype))
-    if n < 1 or x.shape[1] < 1:
-        raise ValueError(f"{name}: weight of shape {tuple(w.shape)}")
-    checks.matrix_dims(name, m, n, x.shape[1])
-    if bias is not None:
-        checks.vec32(bias, f"{name}: bias", n)
-    checks.same_device(name, x, w=w, y=y, bias=bias, addend=addend, preact=preact)
-    checks.overlap(name, y, addend=addend)
-    for k, o in (("y", y), ("preact", preact)):
-        for j, t in (("x", x), ("w", w)):
-            if o is not None and o.numel() and t.numel() and o.data_ptr() == t.data_ptr():
-                raise ValueError(f"{name}: {k} may not be {j}")
-            if o is not None:
-                checks.overlap(name, o, **{j: t})
-    if preact is not None:
-        checks.overlap(name, preact, addend=addend, y=y)
-        if preact.numel() and preact.data_ptr() == y.data_ptr():
-            raise ValueError(f"{name}: preact may not be y")
-    return ld
-
-
-def check_linear_dgrad(dy, w, dx, act, preact, addend):
-    """Row strides (dy, w, dx, preact, addend)."""
-    from . import checks
-    name = "linear_dgrad"
-    if dy.dtype not in checks.FLOATS:
-        raise ValueError(f"{name}: dy must be fp32 or bf16, got {dy.dtype}")
-    ld = [checks.mat(dy, f"{name}: dy"), checks.mat(w, f"{name}: w", dy.shape[1], None, dy.dtype)]
-    m, k = dy.shape[0], w.shape[1]
-    if checks.act_id(act) and preact is None:
-        raise ValueError(f"{name}: act {act!r} needs preact")
-    if not checks.act_id(act) and preact is not None:
-        raise ValueError(f"{name}: preact without an activation")
-    for key, t in (("dx", dx), ("preact", preact), ("addend", addend)):
-        ld.append(0 if t is None else checks.mat(t, f"{name}: {key}", m, k, dy.dtype))
-    if k < 1 or dy.shape[1] < 1:
-        raise ValueError(f"{name}: weight of shape {tuple(w.shape)}")
-    checks.matrix_dims(name, m, k, dy.shape[1])
-    checks.same_device(name, dy, w=w, dx=dx, preact=preact, addend=addend)
-    checks.overlap(name, dx, preact=preact, addend=addend)
-    for key, t in (("dy", dy), ("w", w)):
-        if dx.numel() and t.numel() and dx.data_ptr() == t.data_ptr():
-            raise ValueError(f"{name}: dx may not be {key}")
-        checks.overlap(name, dx, **{key: t})
-    return ld
-
-
-def check_linear_wgrad(dy, x, dw, db):
-    """Row strides (dy, x, dw)."""
-    from . import checks
-    name = "linear_wgrad"
-    if dy.dtype not in checks.FLOATS:
-        raise ValueError(f"{name}: dy must be fp32 or bf16, got {dy.dtype}")
-    ld = [checks.mat(dy, f"{name}: dy"), checks.mat(x, f"{name}: x", dy.shape[0], None, dy.dtype)]
-    n, k = dy.shape[1], x.shape[1]
-    if n < 1 or k < 1:
-        raise ValueError(f"{name}: no columns ({tuple(dy.shape)}, {tuple(x.shape)})")
-    ld.append(checks.mat(dw, f"{name}: dw", n, k, torch.float32))
-    checks.matrix_dims(name, n, k, dy.shape[0])
-    if db is not None:
-        checks.vec32(db, f"{name}: db", n)
-    checks.same_device(name, dy, x=x, dw=dw, db=db)
-    for key, t in (("dy", dy), ("x", x), ("db", db)):
-        if t is not None and t.numel() and dw.data_ptr() == t.data_ptr():
-            raise ValueError(f"{name}: dw may not be {key}")
-        checks.overlap(name, dw, **{key: t})
-    return ld
-
-
 def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
     """y = act(x W^T + bias + addend) for x [M, in] and w [out, in] (both fp32 or both bf16, rows of any stride), bias fp32
     [out].  preact receives the value in front of the activation, which linear_dgrad of the layer behind takes.  y or
     preact may be addend itself."""
-    check_linear_fprop(x, w, y, bias, act, addend, preact)
+    from . import checks
+    checks.linear_fprop(x, w, y, bias, act, addend, preact)
     u = x.float() @ w.float().t()
     if bias is not None:
         u = u + bias
@@ -717,7 +609,8 @@ def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
     """dx = (dy W + addend) * act'(preact) for dy [M, out] and w [out, in]: the gradient in front of the activation whose
     output was this layer's input, with the gradients that other readers of it left in addend.  dx may be addend or preact
     itself."""
-    check_linear_dgrad(dy, w, dx, act, preact, addend)
+    from . import checks
+    checks.linear_dgrad(dy, w, dx, act, preact, addend)
     d = dy.float() @ w.float()
     if addend is not None:
         d = d + addend.float()
@@ -729,7 +622,8 @@ def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
 
 def linear_wgrad(dy, x, dw, db=None, accumulate=False):
     """dw = dy^T x (fp32 [out, in]) and db = the column sums of dy (fp32 [out]); accumulate adds to what they hold."""
-    check_linear_wgrad(dy, x, dw, db)
+    from . import checks
+    checks.linear_wgrad(dy, x, dw, db)
     w, b = dy.float().t() @ x.float(), dy.float().sum(0)
     if accumulate:
         dw.add_(w)
@@ -766,8 +660,7 @@ def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
     groups[group_ids[i]] (fp32 [rows, 2]; uint8, one for each 64 elements).  p16: the bf16 compute copy, or None."""
     from . import checks
     n = p.numel()
-    hi = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi,
-                      {"m": (m, torch.float32, n), "v": (v, torch.float32, n)})
+    hi, _ = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi, (("m", m, torch.float32, n), ("v", v, torch.float32, n)))
     m[lo:hi], v[lo:hi] = _adamw_update(p, g, m[lo:hi].clone(), v[lo:hi].clone(), p16, hyper, groups, group_ids, lo, hi)
 
 
@@ -815,9 +708,9 @@ def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, see
     rounded stochastically with numbers that depend on seed, the step in hyper and the element's index alone."""
     n = p.numel()
     from . import checks
-    hi = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
-                      {"m": (m, torch.float8_e4m3fn, n), "v": (v, torch.float8_e5m2, n),
-                       "m_scale": (m_scale, torch.float32, n // 64), "v_scale": (v_scale, torch.float32, n // 64)})
+    hi, _ = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
+                         (("m", m, torch.float8_e4m3fn, n), ("v", v, torch.float8_e5m2, n), ("m_scale", m_scale, torch.float32, n // 64),
+                          ("v_scale", v_scale, torch.float32, n // 64)))
     bl = slice(lo // 64, hi // 64)
     mm, vv = _adamw_update(p, g, adamw8_decode(m[lo:hi], m_scale[bl]), adamw8_decode(v[lo:hi], v_scale[bl]), p16, hyper, groups,
                            group_ids, lo, hi)
