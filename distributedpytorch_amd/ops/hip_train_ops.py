@@ -124,14 +124,31 @@ def _cdiv(a, b):
 
 
 def _plan(rows, cols, k, f32):
-    """(tile of lin_tile, splits of the reduction)"""
-    if _cdiv(rows, 256) * _cdiv(cols, 256) >= 200:
+    """(tile of lin_tile, splits of the reduction).  The largest tile that still fills the chip: 256 x 256 runs one block on
+    each of the 256 CUs, 128 x 128 two (or one with four steps in LDS), 64 x 64 two.  Measured on both sides, us:
+      256 x 256 below K = 384 pays more for its epilogue than it saves (2909 x 6280 x 192: 28.7, 128 x 128 23.8; 10382 x 5456
+        x 480: 80.6, 94.1); fp32 walks over K six times and has no such bound;
+      128 x 128 from 140 tiles on (1433 x 1872 x 2640, 180 tiles: 36.6, 64 x 64 44.1; 715 x 560 x 1504, 30 tiles: 19, 13.4);
+        two blocks a CU above 256 tiles (6306 x 1112 x 736: 22.6, one 28.8), four steps in LDS below (2048^3: 28.6, 30.4);
+      fp32 in tiles of 128 x 128 has one block a CU, so the last round has to be well filled (688 x 5688 x 888, 270 tiles:
+        88.7, 64 x 64 69.9), and a long reduction is split over it (976 x 744 x 5741: 84.8, 64 x 64 105.8);
+      a split costs a pass over its partial products and pays from 512 elements a part on (3119 x 280 x 624: 9.6 whole, 15.8
+        in two; 784 x 184 x 4670: 15.7 in six, 25 whole; 792 x 1424 x 6161 in 128 x 128: 36.8 in six, 57.8 in whole 64 x 64),
+        in fp32 with few tiles from 128 on (176 x 248 x 571: 13.6 in four, 16.8 whole)."""
+    if _cdiv(rows, 256) * _cdiv(cols, 256) >= 200 and (f32 or k >= 384):
         return 0, 1
-    t128 = _cdiv(rows, 128) * _cdiv(cols, 128)
-    if t128 >= 200:
-        return (4 if f32 else 1 if t128 > 256 else 2), 1
-    t64 = _cdiv(rows, 64) * _cdiv(cols, 64)
-    return (5 if f32 else 3), max(1, min(512 // t64, k // 256, 16))
+    t128, t64 = _cdiv(rows, 128) * _cdiv(cols, 128), _cdiv(rows, 64) * _cdiv(cols, 64)
+    if f32:
+        if t128 >= 160 * _cdiv(t128, 256):
+            return 4, 1
+        if 40 <= t128 <= 128 and k >= 1500:
+            return 4, min(256 // t128, k // 512)
+        return 5, max(1, min(512 // t64, k // (128 if t64 < 64 else 384), 16))
+    if k >= 4096 and 32 <= t128 < 200:
+        return 1, min(512 // t128, k // 768, 16)
+    if t128 >= 140:
+        return (1 if t128 > 256 else 2), 1
+    return 3, max(1, min(512 // t64, k // 512, 16))
 
 
 def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
@@ -145,7 +162,8 @@ def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
     c.vec_a = ok_a = not (a[0] | a[1] * es) & 15
     c.vec_b = ok_b = not (b[0] | b[1] * es) & 15
     c.K, c.parts = k, 3 if f32 else 1
-    few = c.epi == _FPROP and c.rows <= 64 and ok_a and ok_b and not (k * es) & 15
+    few = c.epi == _FPROP and c.rows <= (64 if f32 else 32) and ok_a and ok_b and not (k * es) & 15
+    # (32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
     c.a, c.lda, c.b, c.ldb = a[0], a[1], b[0], b[1]
     need = 0
     if few:
