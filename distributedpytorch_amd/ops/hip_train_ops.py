@@ -7,6 +7,7 @@ is one call into the library."""
 from __future__ import annotations
 
 import ctypes
+import math
 from ctypes import byref
 
 import torch
@@ -21,7 +22,8 @@ class GnParams(ctypes.Structure):
     _fields_ = [("x", VP), ("res", VP), ("dy", VP), ("yv", VP), ("y", VP), ("dx", VP), ("dres", VP), ("gamma", VP), ("beta", VP),
                 ("mean", VP), ("rstd", VP), ("slab", VP), ("coef", VP), ("dgamma", VP), ("dbeta", VP),
                 ("x_cs", I64), ("res_cs", I64), ("dy_cs", I64), ("yv_cs", I64), ("y_cs", I64), ("dx_cs", I64), ("dres_cs", I64),
-                ("N", I32), ("HW", I32), ("C", I32), ("G", I32), ("cg", I32), ("S", I32), ("pps", I32), ("eps", F32)]
+                ("N", I32), ("HW", I32), ("C", I32), ("G", I32), ("cg", I32), ("S", I32), ("pps", I32),
+                ("act", I32), ("W", I32), ("rows", I32), ("R", I32), ("threads", I32), ("way", I32), ("eps", F32)]
 
 
 class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
@@ -56,34 +58,86 @@ def _run(device, body, *args):
         return body(VP(torch._C._cuda_getCurrentRawStream(i)), *args)
 
 
+def _cdiv(a, b):
+    return (a + b - 1) // b
+
+
 # ----------------------------------------------------------------------------------------- group norm
-def _gn_splits(n, hw, c):
-    """Pixel ranges per image: enough blocks for 256 CUs where there are few images and channels."""
-    blocks = n * ((c + 63) // 64)
-    s = max(1, min((hw + 15) // 16, 2048 // max(blocks, 1), 64))
-    pps = (hw + s - 1) // s
-    return (hw + pps - 1) // pps, pps
+_ANY, _ONE, _TWO = 0, 1, 2          # csrc/hip/group_norm.hip
+_plans = {}
 
 
-def _gn_params(x, groups, vecs):
+def _gn_plan(n, hw, c, cg, v, bwd):
+    """(way, threads, W, rows, R, S, pixels of a split) of csrc/hip/group_norm.hip for vectors of v channels (0: any layout).
+
+    A block that holds its chunk of an image in registers reads everything once, so it is taken wherever an image fits: the
+    chunk as wide as possible, down to 32 bytes of a pixel (times in us, relu + residual, 64 images, bf16; the other side is
+    two passes): 40 x 40 x 256 forward in 128 bytes 37.0, 64 bytes 40.2, two passes 52.7, backward in 64 bytes 73.6, two passes
+    124.4; 56 x 56 x 256 forward in 64 bytes 79.7, two passes 88.3, backward in 32 bytes 184, two passes 229.
+    Few images make too few blocks: then the chunk is as narrow as it goes (4 images of 28 x 28 x 512: 7.1 forward and 15.1
+    backward, 10.5 and 21.3 in 128 bytes), and a large image goes through two passes (4 of 56 x 56 x 256: 15.5 and 25.9, one
+    pass 19.9 and 30.4; with 16 images 26.3 and 69.2, one pass 21.7 and 49.5)."""
+    if v:
+        unit = cg * v // math.gcd(cg, v) // v          # vectors of the smallest chunk of whole groups
+        total = c // v
+        chunks = [w for w in range(unit, min(total, 256) + 1, unit) if total % w == 0]
+        sizes = ((256, 1), (256, 2), (512, 4), (512, 7), (512, 13)) + (() if bwd else ((1024, 13),))
+        for want in (8, 4, 2) if n * (total // 8) >= 128 else (2,):
+            for threads, r in sizes:
+                for w in chunks:
+                    if (w >= want or w == chunks[-1]) and w <= threads and hw <= threads // w * r and w * v // cg <= 1024:
+                        if hw > 1024 and n * (total // w) < 256:
+                            break
+                        return _ONE, threads, w, threads // w, r, 1, hw
+        fit = [w for w in chunks if w * v // cg <= 1024]
+        if fit:
+            w = next((w for w in fit if w >= 16), fit[-1])
+            rows, r = 512 // w, 2 if bwd else 8
+            pps = rows * r * (max(1, n * _cdiv(hw, rows * r) * (total // w) // 1024) if bwd else 1)
+            return _TWO, 512, w, rows, r, _cdiv(hw, pps), pps
+    blocks = n * _cdiv(c, 64)
+    s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64))
+    pps = _cdiv(hw, s)
+    return _ANY, 256, 1, 1, 1, _cdiv(hw, pps), pps
+
+
+def _gn(x, groups, vecs, spans, bwd, a, eps=0.0):
     n, h, w, c = x.shape
     p = GnParams()
     p.gamma, p.beta, p.mean, p.rstd = vecs[:4]
-    p.N, p.HW, p.C, p.G, p.cg = n, h * w, c, groups, c // groups
-    p.S, p.pps = _gn_splits(n, h * w, c)
+    f32 = x.dtype is _F32
+    v, bits = (4 if f32 else 8), 0
+    for s in spans:
+        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 20)          # (offsets of a lane in 32 bits)
+    key = (n, h * w, c, groups, 0 if bits & 15 or c % v else v, bwd)
+    plan = _plans.get(key)
+    if plan is None:
+        if len(_plans) > 4096:
+            _plans.clear()
+        plan = _plans[key] = _gn_plan(n, h * w, c, c // groups, key[4], bwd)
+    p.N, p.HW, p.C, p.G, p.cg, p.act, p.eps = n, h * w, c, groups, c // groups, a, eps
+    p.way, p.threads, p.W, p.rows, p.R, p.S, p.pps = plan
     return p
+
+
+def _gn_launch(stream, p, x, slab, coef, bwd):
+    ws = torch.empty(slab + coef, device=x.device, dtype=_F32) if slab + coef else None
+    if ws is not None:
+        p.slab = ws.data_ptr()
+        p.coef = p.slab + 4 * slab
+    _lib().dpa_group_norm(byref(p), bwd, int(x.dtype is _F32), stream)
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", residual=None):
     a, xs, ys, rs, vecs = checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
     if x.numel() == 0:
         return y
-    p = _gn_params(x, groups, vecs)
+    p = _gn(x, groups, vecs, (xs, ys, rs), 0, a, eps)
     p.x, p.x_cs, _ = xs
     p.y, p.y_cs, _ = ys
     p.res, p.res_cs, _ = rs
-    p.eps = eps
-    _run(x.device, _gn_launch, p, x, p.N * p.S * 2 * p.C, _lib().dpa_group_norm_fwd, a)
+    slab = 0 if p.way == _ONE else p.N * p.S * 2 * (p.G if p.way == _TWO else p.C)
+    _run(x.device, _gn_launch, p, x, slab, 0, 0)
     return y
 
 
@@ -96,7 +150,7 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
             if t is not None:
                 t.zero_()
         return dx
-    p = _gn_params(x, groups, vecs)
+    p = _gn(x, groups, vecs, (xs, dys, dxs, ys, rs, drs), 1, a)
     p.dgamma, p.dbeta = vecs[4:]
     p.x, p.x_cs, _ = xs
     p.dy, p.dy_cs, _ = dys
@@ -104,23 +158,14 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
     p.yv, p.yv_cs, _ = ys
     p.res, p.res_cs, _ = rs
     p.dres, p.dres_cs, _ = drs
-    _run(x.device, _gn_launch, p, x, p.N * p.S * 2 * p.C, _lib().dpa_group_norm_bwd, a)
+    slab = p.N * p.S * 2 * p.C if p.way == _ANY or dgamma is not None or dbeta is not None else 0
+    coef = 0 if p.way == _ONE else 2 * p.N * p.G * (p.S if p.way == _TWO else 1)
+    _run(x.device, _gn_launch, p, x, slab, coef, 1)
     return dx
-
-
-def _gn_launch(stream, p, x, slab, entry, act):
-    ws = torch.empty(slab + 2 * p.N * p.G, device=x.device, dtype=_F32)
-    p.slab = ws.data_ptr()
-    p.coef = p.slab + 4 * slab
-    entry(byref(p), act, int(x.dtype is _BF16), stream)
 
 
 # ----------------------------------------------------------------------------------------- linear products
 _FPROP, _DGRAD, _WGRAD = 0, 1, 2          # csrc/hip/linear.h
-
-
-def _cdiv(a, b):
-    return (a + b - 1) // b
 
 
 def _plan(rows, cols, k, f32):
