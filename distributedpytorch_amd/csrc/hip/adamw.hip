@@ -7,23 +7,46 @@
 // Every tensor of the arena starts at a multiple of 64 elements; group_ids[i] names the row (lr multiplier, decay
 // multiplier) of `groups` that the i-th run of 64 elements uses.  `hyper` is the vector of optim.hip (slots at its top): in
 // device memory, so a captured graph follows lr and step.
+//
+// Both kernels are bound by memory: one read and one write of every operand, 30 bytes a parameter with 32-bit
+// states and 18.25 with 8-bit ones (p 8, g 4, p16 2, states 16, or 4 and 0.25 of scales).  Operands that no kernel reads before the next step, larger together than
+// the caches, pass them by (nontemporal), and many short-lived blocks keep more requests in flight than 2048 long ones: 25.6
+// million parameters with p16 159 us in 2048 blocks with cached accesses, 147 in 16384, 133 (5.8 TB/s) with nontemporal ones.
+// The 8-bit kernel computes some 110 instructions an element beside its bytes: 132.9 million parameters 528 us with
+// IEEE square roots, divisions and rounding by ldexp in 2048 blocks, 499 in 16384, 460 (5.3 TB/s) with the forms below; one
+// block a vector, or 4 elements a lane, was no faster (458, 487).
 #include "common.h"
+#include <algorithm>
 
-struct AdamwScalars { float lr, wd, b2, eps, gs, omb1, omb2, inv_bc1, bc2s; };
+typedef __attribute__((ext_vector_type(4))) float adamw_f4;
+__device__ __forceinline__ float4 adamw_ld(const float* q) { return __builtin_bit_cast(float4, __builtin_nontemporal_load((const adamw_f4*)q)); }
+__device__ __forceinline__ void adamw_st(float* q, float4 x) { __builtin_nontemporal_store(__builtin_bit_cast(adamw_f4, x), (adamw_f4*)q); }
+static int adamw_grid(long long threads) { return (int)std::min<long long>(16384, (threads + 255) / 256); }
+
+struct AdamwScalars { float lr, wd, b2, eps, gs, omb1, omb2, inv_bc1, bc2s, inv_bc2s; };
 
 __device__ __forceinline__ AdamwScalars adamw_scalars(const float* __restrict__ h) {
   AdamwScalars a;
   a.lr = h[0]; a.wd = h[4]; a.b2 = h[2]; a.eps = h[3]; a.gs = h[7]; a.omb1 = h[8]; a.omb2 = h[9];
   const double t = (double)h[5] + 1.0, b1 = (double)h[1] + (double)h[10], b2 = (double)h[2] + (double)h[11];
   a.inv_bc1 = (float)(1.0 / (1.0 - pow(b1, t)));
-  a.bc2s = (float)sqrt(1.0 - pow(b2, t));
+  const double bc2s = sqrt(1.0 - pow(b2, t));
+  a.bc2s = (float)bc2s;
+  a.inv_bc2s = (float)(1.0 / bc2s);
   return a;
 }
 
+// FAST: square root and reciprocal of the hardware, one unit in the last place each, of an update that is added to a parameter
+template <bool FAST>
 __device__ __forceinline__ float adamw_one(const AdamwScalars& a, float lr, float keep, float p, float g, float& m, float& v) {
   g *= a.gs;
   m += a.omb1 * (g - m);
   v = a.b2 * v + a.omb2 * g * g;
+  if (FAST) {
+    const bool small = v < 0x1p-96f;          // (the hardware's root of a denormal number is 0)
+    const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.f);
+    return p * keep - (lr * a.inv_bc1) * (m * __builtin_amdgcn_rcpf(root * a.inv_bc2s + a.eps));
+  }
   return p * keep - (lr * a.inv_bc1) * (m / (sqrtf(v) / a.bc2s + a.eps));
 }
 
@@ -36,12 +59,12 @@ __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const
   for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < n; i += stride) {      // n % 64 == 0
     const float2 grp = groups[ids[i >> 6]];
     const float lr = a.lr * grp.x, keep = 1.f - lr * (a.wd * grp.y);
-    float4 pp = *(float4*)(p + i), mm = *(float4*)(m + i), vv = *(float4*)(v + i);
-    const float4 gg = *(const float4*)(g + i);
+    float4 pp = adamw_ld(p + i), mm = adamw_ld(m + i), vv = adamw_ld(v + i);
+    const float4 gg = adamw_ld(g + i);
     float* pa = (float*)&pp; float* ma = (float*)&mm; float* va = (float*)&vv; const float* ga = (const float*)&gg;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) pa[k] = adamw_one(a, lr, keep, pa[k], ga[k], ma[k], va[k]);
-    *(float4*)(p + i) = pp; *(float4*)(m + i) = mm; *(float4*)(v + i) = vv;
+    for (int k = 0; k < 4; ++k) pa[k] = adamw_one<false>(a, lr, keep, pa[k], ga[k], ma[k], va[k]);
+    adamw_st(p + i, pp); adamw_st(m + i, mm); adamw_st(v + i, vv);
     if (p16) {
       uint2 o;
       o.x = (uint32_t)f2bf(pa[0]) | ((uint32_t)f2bf(pa[1]) << 16);
@@ -65,15 +88,16 @@ __device__ __forceinline__ uint32_t adamw_mix(uint32_t h) {        // finalizer 
   return h ^ (h >> 16);
 }
 
-// |t| * inv rounded to a multiple of its binade's step, with u in (0, 1): the magnitude of the code
+// |t| * inv rounded to a multiple of its binade's step, up with the probability of the remainder: the 16 random bits and a
+// half are added to the mantissa bits below the step, which are cut off.  Below 2^LEAST the step stays the same: 2^LEAST is
+// added first and taken off again.  (The largest value `top` has no bits below its step, so nothing is rounded above it.)
 template <int LEAST, int BITS>
-__device__ __forceinline__ float adamw_round(float t, float inv, float top, float u) {
+__device__ __forceinline__ float adamw_round(float t, float inv, float top, uint32_t r16) {
   float y = fabsf(t) * inv;
   y = y < top ? y : top;                                   // (also NaN)
-  int e = ilogbf(y);
-  e = (y == 0.f || e < LEAST) ? LEAST : e;
-  const float q = ldexpf(floorf(ldexpf(y, BITS - e) + u), e - BITS);
-  return q < top ? q : top;
+  const float least = __uint_as_float((uint32_t)(LEAST + 127) << 23), base = y < least ? least : 0.f;
+  const uint32_t q = __float_as_uint(y + base) + (r16 << (7 - BITS)) + (1u << (6 - BITS));
+  return __uint_as_float(q & ~((1u << (23 - BITS)) - 1)) - base;
 }
 
 __device__ __forceinline__ float adamw_block_max(float a) {        // over the 8 lanes that share a block
@@ -110,7 +134,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      pa[k] = adamw_one(a, lr, keep, pa[k], ga[k], mv[k], vv[k]);
+      pa[k] = adamw_one<true>(a, lr, keep, pa[k], ga[k], mv[k], vv[k]);
       const float x = fabsf(mv[k]), y = fabsf(vv[k]);
       am = fmaxf(am, x < INFINITY ? x : 0.f);
       av = fmaxf(av, y < INFINITY ? y : 0.f);
@@ -126,8 +150,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
       for (int j = 0; j < 2; ++j) {
         const unsigned long long at = (unsigned long long)(first + i + k + j);
         const uint32_t r = adamw_mix((uint32_t)at ^ key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu));
-        qm[j] = copysignf(adamw_round<-6, 3>(mv[k + j], im, 448.f, ((float)(r & 0xFFFFu) + 0.5f) * 0x1p-16f), mv[k + j]);
-        qv[j] = adamw_round<-14, 2>(vv[k + j], iv, 57344.f, ((float)(r >> 16) + 0.5f) * 0x1p-16f);
+        qm[j] = copysignf(adamw_round<-6, 3>(mv[k + j], im, 448.f, r & 0xFFFFu), mv[k + j]);
+        qv[j] = adamw_round<-14, 2>(vv[k + j], iv, 57344.f, r >> 16);
         if (vv[k + j] > 0.f && some_v) qv[j] = fmaxf(qv[j], 0x1p-16f);
       }
       // (both values are representable: these conversions round nothing)
@@ -155,14 +179,14 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
 DPA_API int dpa_adamw_step(float* p, const float* g, float* m, float* v, bf16_t* p16, const float* hyper, const float* groups,
                            const unsigned char* ids, long long n, hipStream_t s) {
   if (n <= 0) return 0;
-  hipLaunchKernelGGL(adamw_kernel, dim3(dpa_grid(n / 4, 256)), dim3(256), 0, s, p, g, m, v, p16, hyper, (const float2*)groups, ids, n);
+  hipLaunchKernelGGL(adamw_kernel, dim3(adamw_grid(n / 4)), dim3(256), 0, s, p, g, m, v, p16, hyper, (const float2*)groups, ids, n);
   return dpa_launch_rc();
 }
 DPA_API int dpa_adamw8_step(float* p, const float* g, unsigned char* m8, unsigned char* v8, float* ms, float* vs, bf16_t* p16,
                             const float* hyper, const float* groups, const unsigned char* ids, unsigned int seed, long long first,
                             long long n, hipStream_t s) {
   if (n <= 0) return 0;
-  hipLaunchKernelGGL(adamw8_kernel, dim3(dpa_grid(n / 8, 256)), dim3(256), 0, s, p, g, m8, v8, ms, vs, p16, hyper,
+  hipLaunchKernelGGL(adamw8_kernel, dim3(adamw_grid(n / 8)), dim3(256), 0, s, p, g, m8, v8, ms, vs, p16, hyper,
                      (const float2*)groups, ids, seed, first, n);
   return dpa_launch_rc();
 }
