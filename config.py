@@ -39,7 +39,9 @@ MASTER_PORT = _env("MASTER_PORT", '6779')
 
 MODEL_NAME = _env("MODEL_NAME", 'resnet')  # resnet | alexnet | vgg | squeezenet | densenet | inception (| resnet50 | basic)
 
-OPTIMIZER = _env("OPTIMIZER", 'adam')  # adam | SGD
+OPTIMIZER = _env("OPTIMIZER", 'adam')  # adam | SGD | adamw (decoupled weight decay on matrices and filters) | adamw8 (the same, states of 8 bits)
+
+WEIGHT_DECAY = _env("WEIGHT_DECAY", 0.01, float)   # of adamw and adamw8
 
 LOSS = _env("LOSS", 'cross_entropy')  # cross_entropy | weighted_cross_entropy | focal_loss
 
@@ -74,6 +76,9 @@ FIRST_BUCKET_MB = _env("FIRST_BUCKET_MB", 1.0, float)    # DDP first (last-layer
 BUCKET_CAP_MB = _env("BUCKET_CAP_MB", 25.0, float)       # DDP bucket cap: torch DDP's default, NOT yet swept on an 8-GPU node (scripts/allreduce_bench.py --sweep does it; SURVEY.md §5.8 expects 16-32 MiB to keep each of the 7 xGMI links bandwidth-bound)
 BROADCAST_BUFFERS = _env("BROADCAST_BUFFERS", True, bool)  # DDP semantics: rank 0's BatchNorm statistics win every step
 COMM_BACKEND = _env("COMM_BACKEND", 'native')      # native (default: C++ store rendezvous + ONE native communicator per rank - RCCL over xGMI on GPUs, TCP mesh on CPUs; csrc/comm) | torch (fallback: torch.distributed RCCL process group / gloo)
+NORM = _env("NORM", 'batch')                       # resnet, resnet50: batch (batch statistics) | group (32 groups of channels of each image: nothing to exchange between ranks, nothing that depends on the batch)
+ACT = _env("ACT", 'relu')                          # activation of a network with NORM=group and of its classifier: relu | silu | gelu
+HEAD_HIDDEN = _env("HEAD_HIDDEN", '')              # resnet, resnet50: widths of hidden layers of the classifier, e.g. "1024,512"
 USE_HIPGRAPH = _env("USE_HIPGRAPH", True, bool)   # replay the training iteration from a hipGraph when world_size == 1
 SYNC_COMM = _env("SYNC_COMM", False, bool)        # debug: synchronous collectives (race-detection aid)
 GLOBAL_METRICS = _env("GLOBAL_METRICS", False, bool)  # all-reduce (loss, acc) over ranks; False = reference behaviour

@@ -5,8 +5,8 @@
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
 // Every tensor of the arena starts at a multiple of 64 elements; group_ids[i] names the row (lr multiplier, decay
-// multiplier) of `groups` that the i-th run of 64 elements uses.  `hyper` is the vector of optim.hip (slots at its top): in
-// device memory, so a captured graph follows lr and step.
+// multiplier) of `groups` that the i-th run of 64 elements uses; the last row stands in for rows that are not there.  `hyper`
+// is the vector of optim.hip (slots at its top): in device memory, so a captured graph follows lr and step.
 //
 // Both kernels are bound by memory: one read and one write of every operand, 30 bytes a parameter with 32-bit
 // states and 18.25 with 8-bit ones (p 8, g 4, p16 2, states 16, or 4 and 0.25 of scales).  Operands that no kernel reads before the next step, larger together than
@@ -52,12 +52,12 @@ __device__ __forceinline__ float adamw_one(const AdamwScalars& a, float lr, floa
 
 __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                                                     float* __restrict__ v, bf16_t* __restrict__ p16,
-                                                    const float* __restrict__ hyper, const float2* __restrict__ groups,
+                                                    const float* __restrict__ hyper, const float2* __restrict__ groups, int rows,
                                                     const unsigned char* __restrict__ ids, long long n) {
   const AdamwScalars a = adamw_scalars(hyper);
   const long long stride = (long long)gridDim.x * blockDim.x * 4;
   for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < n; i += stride) {      // n % 64 == 0
-    const float2 grp = groups[ids[i >> 6]];
+    const float2 grp = groups[min((int)ids[i >> 6], rows - 1)];
     const float lr = a.lr * grp.x, keep = 1.f - lr * (a.wd * grp.y);
     float4 pp = adamw_ld(p + i), mm = adamw_ld(m + i), vv = adamw_ld(v + i);
     const float4 gg = adamw_ld(g + i);
@@ -108,14 +108,14 @@ __device__ __forceinline__ float adamw_block_max(float a) {        // over the 8
 __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, const float* __restrict__ g, unsigned char* __restrict__ m8,
                                                      unsigned char* __restrict__ v8, float* __restrict__ ms, float* __restrict__ vs,
                                                      bf16_t* __restrict__ p16, const float* __restrict__ hyper,
-                                                     const float2* __restrict__ groups, const unsigned char* __restrict__ ids,
-                                                     uint32_t seed, long long first, long long n) {
+                                                     const float2* __restrict__ groups, int rows,
+                                                     const unsigned char* __restrict__ ids, uint32_t seed, long long first, long long n) {
   const AdamwScalars a = adamw_scalars(hyper);
   const uint32_t key = adamw_mix(seed + (uint32_t)(long long)hyper[5] * 0x9E3779B9u);
   const long long stride = (long long)gridDim.x * blockDim.x * 8;
   for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < n; i += stride) {      // whole blocks of 8 lanes
     const long long b = i >> 6;
-    const float2 grp = groups[ids[b]];
+    const float2 grp = groups[min((int)ids[b], rows - 1)];
     const float lr = a.lr * grp.x, keep = 1.f - lr * (a.wd * grp.y);
     const float sm = ms[b], sv = vs[b];
     float4 pp[2], gg[2];
@@ -176,17 +176,17 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
   }
 }
 
-DPA_API int dpa_adamw_step(float* p, const float* g, float* m, float* v, bf16_t* p16, const float* hyper, const float* groups,
+DPA_API int dpa_adamw_step(float* p, const float* g, float* m, float* v, bf16_t* p16, const float* hyper, const float* groups, int rows,
                            const unsigned char* ids, long long n, hipStream_t s) {
   if (n <= 0) return 0;
-  hipLaunchKernelGGL(adamw_kernel, dim3(adamw_grid(n / 4)), dim3(256), 0, s, p, g, m, v, p16, hyper, (const float2*)groups, ids, n);
+  hipLaunchKernelGGL(adamw_kernel, dim3(adamw_grid(n / 4)), dim3(256), 0, s, p, g, m, v, p16, hyper, (const float2*)groups, rows, ids, n);
   return dpa_launch_rc();
 }
 DPA_API int dpa_adamw8_step(float* p, const float* g, unsigned char* m8, unsigned char* v8, float* ms, float* vs, bf16_t* p16,
-                            const float* hyper, const float* groups, const unsigned char* ids, unsigned int seed, long long first,
+                            const float* hyper, const float* groups, int rows, const unsigned char* ids, unsigned int seed, long long first,
                             long long n, hipStream_t s) {
   if (n <= 0) return 0;
   hipLaunchKernelGGL(adamw8_kernel, dim3(adamw_grid(n / 8)), dim3(256), 0, s, p, g, m8, v8, ms, vs, p16, hyper,
-                     (const float2*)groups, ids, seed, first, n);
+                     (const float2*)groups, rows, ids, seed, first, n);
   return dpa_launch_rc();
 }

@@ -62,20 +62,24 @@ class Network:
 
 
 def get_model(model_name, num_classes, feature_extract=False, use_pretrained=False, device="cpu",
-              dtype=torch.float32, small_input=False):
+              dtype=torch.float32, small_input=False, norm="batch", act="relu", head_hidden=()):
     """utils.getModel equivalent.  Returns (Network, input_size).  `use_pretrained` needs torchvision weights, which
-    cannot be downloaded here (no network): it is accepted for interface parity and rejected if True."""
+    cannot be downloaded here (no network): it is accepted for interface parity and rejected if True.
+    norm, act, head_hidden: of the ResNets (models/resnet.py); other models take their defaults only."""
     if use_pretrained:
         raise RuntimeError("USE_PRETRAINED=True needs downloadable torchvision weights; load a checkpoint with -f instead")
+    kw = dict(norm=norm, act=act, head_hidden=tuple(head_hidden))
+    if model_name not in ("resnet", "resnet50") and (norm != "batch" or act != "relu" or kw["head_hidden"]):
+        raise ValueError(f"norm, act and head_hidden belong to the ResNets, not to {model_name!r}")
     store = ParamStore(device, dtype)
     from ..nn import layers as _layers
     _layers._dropout_ids[0] = 0          # dropout stream ids are per model: two identical builds draw identical masks
     if model_name == "resnet":
         from .resnet import resnet18
-        net = resnet18(store, num_classes, feature_extract, small_input)
+        net = resnet18(store, num_classes, feature_extract, small_input, **kw)
     elif model_name == "resnet50":
         from .resnet import resnet50
-        net = resnet50(store, num_classes, feature_extract, small_input)
+        net = resnet50(store, num_classes, feature_extract, small_input, **kw)
     elif model_name == "alexnet":
         from .alexnet import alexnet
         net = alexnet(store, num_classes, feature_extract)

@@ -7,8 +7,9 @@ from __future__ import annotations
 import os
 
 from ..nn.engine import Act, Context, ParamStore
-from ..nn.layers import (AvgPool2d, BatchNorm2d, Conv2d, ConvBNAct, ConvBNReLUPool, Linear, MaxPool2d,
-                         kaiming_normal_fan_out)
+from ..nn.layers import (AvgPool2d, BatchNorm2d, Conv2d, ConvBNAct, ConvBNReLUPool, ConvGNAct, GroupNorm2d, Linear, MaxPool2d,
+                         Mlp, kaiming_normal_fan_out)
+from ..ops.checks import ACTS
 
 
 # DPA_FUSE_STEM_POOL=0: stem as conv+BN+ReLU followed by a separate max-pool (A/B switch for nn/layers.py:ConvBNReLUPool)
@@ -21,9 +22,12 @@ _FUSE_STEM_POOL = os.environ.get("DPA_FUSE_STEM_POOL", "1") != "0"
 _DOWN_LAST = os.environ.get("DPA_RESNET_DOWN_LAST", "1") != "0"
 
 
-def _cb(store, prefix, conv_name, bn_name, cin, cout, k, stride, pad, trainable):
+def _cb(store, prefix, conv_name, bn_name, cin, cout, k, stride, pad, trainable, norm="batch", act="relu"):
+    """norm "group": groups of channels of each image instead of batch statistics, under the same parameter names."""
     conv = Conv2d(store, f"{prefix}{conv_name}", cin, cout, k, stride, pad, bias=False, w_init=kaiming_normal_fan_out,
                   trainable=trainable)
+    if norm == "group":
+        return ConvGNAct(conv, GroupNorm2d(store, f"{prefix}{bn_name}", cout, trainable=trainable), act)
     bn = BatchNorm2d(store, f"{prefix}{bn_name}", cout, trainable=trainable)
     return ConvBNAct(conv, bn)
 
@@ -31,12 +35,12 @@ def _cb(store, prefix, conv_name, bn_name, cin, cout, k, stride, pad, trainable)
 class BasicBlock:
     expansion = 1
 
-    def __init__(self, store, prefix, cin, planes, stride, trainable):
-        self.c1 = _cb(store, prefix, "conv1", "bn1", cin, planes, 3, stride, 1, trainable)
-        self.c2 = _cb(store, prefix, "conv2", "bn2", planes, planes, 3, 1, 1, trainable)
+    def __init__(self, store, prefix, cin, planes, stride, trainable, **kw):
+        self.c1 = _cb(store, prefix, "conv1", "bn1", cin, planes, 3, stride, 1, trainable, **kw)
+        self.c2 = _cb(store, prefix, "conv2", "bn2", planes, planes, 3, 1, 1, trainable, **kw)
         self.down = None
         if stride != 1 or cin != planes:
-            self.down = _cb(store, prefix, "downsample.0", "downsample.1", cin, planes, 1, stride, 0, trainable)
+            self.down = _cb(store, prefix, "downsample.0", "downsample.1", cin, planes, 1, stride, 0, trainable, **kw)
 
     def __call__(self, ctx: Context, x: Act, sole_consumer=False) -> Act:
         """sole_consumer: nothing but this block reads x (the caller's promise).  Then conv1's dgrad completes x.grad
@@ -57,13 +61,13 @@ class BasicBlock:
 class Bottleneck:
     expansion = 4
 
-    def __init__(self, store, prefix, cin, planes, stride, trainable):
-        self.c1 = _cb(store, prefix, "conv1", "bn1", cin, planes, 1, 1, 0, trainable)
-        self.c2 = _cb(store, prefix, "conv2", "bn2", planes, planes, 3, stride, 1, trainable)   # v1.5: stride on 3x3
-        self.c3 = _cb(store, prefix, "conv3", "bn3", planes, planes * 4, 1, 1, 0, trainable)
+    def __init__(self, store, prefix, cin, planes, stride, trainable, **kw):
+        self.c1 = _cb(store, prefix, "conv1", "bn1", cin, planes, 1, 1, 0, trainable, **kw)
+        self.c2 = _cb(store, prefix, "conv2", "bn2", planes, planes, 3, stride, 1, trainable, **kw)   # v1.5: stride on 3x3
+        self.c3 = _cb(store, prefix, "conv3", "bn3", planes, planes * 4, 1, 1, 0, trainable, **kw)
         self.down = None
         if stride != 1 or cin != planes * 4:
-            self.down = _cb(store, prefix, "downsample.0", "downsample.1", cin, planes * 4, 1, stride, 0, trainable)
+            self.down = _cb(store, prefix, "downsample.0", "downsample.1", cin, planes * 4, 1, stride, 0, trainable, **kw)
 
     def __call__(self, ctx: Context, x: Act, sole_consumer=False) -> Act:
         if self.down is not None and _DOWN_LAST and sole_consumer and getattr(x, "bn_src", None) is not None:
@@ -79,30 +83,44 @@ class Bottleneck:
 
 
 class ResNet:
-    def __init__(self, store: ParamStore, block, layers, num_classes, feature_extract=False, small_input=False):
+    def __init__(self, store: ParamStore, block, layers, num_classes, feature_extract=False, small_input=False, norm="batch",
+                 act="relu", head_hidden=()):
+        """norm: "batch", or "group" (32 groups; the activation may then be any of ops/checks.py: ACTS).  head_hidden: widths of hidden layers
+        of the classifier, which is then an MLP (nn/layers.py: Mlp); a network with group norms always has one."""
+        if norm not in ("batch", "group"):
+            raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+        if act not in ACTS:
+            raise ValueError(f"act must be one of {tuple(ACTS)}, got {act!r}")
+        if norm == "batch" and act != "relu":
+            raise ValueError(f"batch norms carry a ReLU; act is {act!r}")
+        kw = dict(norm=norm, act=act)
         t = not feature_extract
         self.store = store
         self.num_classes = num_classes
         # small_input: CIFAR-style stem (3x3 stride 1, no max-pool) for 32x32 data (BASELINE.json config 4)
         if small_input:
-            self.stem = _cb(store, "", "conv1", "bn1", 3, 64, 3, 1, 1, t)
+            self.stem = _cb(store, "", "conv1", "bn1", 3, 64, 3, 1, 1, t, **kw)
             self.maxpool = None
         else:
-            self.stem = _cb(store, "", "conv1", "bn1", 3, 64, 7, 2, 3, t)
+            self.stem = _cb(store, "", "conv1", "bn1", 3, 64, 7, 2, 3, t, **kw)
             self.maxpool = MaxPool2d(3, 2, 1)
-            self.stem_pool = ConvBNReLUPool(self.stem.conv, self.stem.bn, self.maxpool)      # fused stem (nn/layers.py)
+            if norm == "batch":
+                self.stem_pool = ConvBNReLUPool(self.stem.conv, self.stem.bn, self.maxpool)      # fused stem (nn/layers.py)
         self.blocks = []
         cin = 64
         for li, (planes, n) in enumerate(zip((64, 128, 256, 512), layers)):
             for bi in range(n):
                 stride = 2 if (bi == 0 and li > 0) else 1
-                self.blocks.append(block(store, f"layer{li + 1}.{bi}.", cin, planes, stride, t))
+                self.blocks.append(block(store, f"layer{li + 1}.{bi}.", cin, planes, stride, t, **kw))
                 cin = planes * block.expansion
         self.avgpool = AvgPool2d(adaptive=1)
-        self.fc = Linear(store, "fc", cin, num_classes, bias=True, trainable=True)
+        if norm == "group" or head_hidden:
+            self.fc = Mlp(store, "fc", (cin, *head_hidden, num_classes), act)
+        else:
+            self.fc = Linear(store, "fc", cin, num_classes, bias=True, trainable=True)
 
     def forward(self, ctx: Context, x: Act):
-        if self.maxpool is not None and _FUSE_STEM_POOL:
+        if _FUSE_STEM_POOL and hasattr(self, "stem_pool"):
             x = self.stem_pool(ctx, x)
         else:
             x = self.stem(ctx, x, relu=True)
@@ -114,9 +132,9 @@ class ResNet:
         return self.fc(ctx, x)
 
 
-def resnet18(store, num_classes, feature_extract=False, small_input=False):
-    return ResNet(store, BasicBlock, (2, 2, 2, 2), num_classes, feature_extract, small_input)
+def resnet18(store, num_classes, feature_extract=False, small_input=False, **kw):
+    return ResNet(store, BasicBlock, (2, 2, 2, 2), num_classes, feature_extract, small_input, **kw)
 
 
-def resnet50(store, num_classes, feature_extract=False, small_input=False):
-    return ResNet(store, Bottleneck, (3, 4, 6, 3), num_classes, feature_extract, small_input)
+def resnet50(store, num_classes, feature_extract=False, small_input=False, **kw):
+    return ResNet(store, Bottleneck, (3, 4, 6, 3), num_classes, feature_extract, small_input, **kw)

@@ -621,6 +621,95 @@ class BNAct:
         return y
 
 
+class GroupNorm2d:
+    """Group normalisation over [N, H, W, C]: statistics of every image's groups of channels, no running statistics, so training
+    and evaluation compute the same and nothing is exchanged between ranks.  Parameter names as in torch's GroupNorm."""
+
+    def __init__(self, store: ParamStore, name, c, groups=32, eps=1e-5, trainable=True):
+        if groups < 1 or c % groups or c != pad_to(c):
+            raise ValueError(f"{name}: {c} channels do not divide into {groups} groups of an unpadded activation")
+        self.store, self.c, self.groups, self.eps = store, c, groups, eps
+        self.gamma = store.add_vec(f"{name}.weight", c, ones_, trainable)
+        self.beta = store.add_vec(f"{name}.bias", c, zeros_, trainable)
+        self.trainable = trainable
+
+    def forward(self, ctx: Context, x, act="none", residual=None, out=None):
+        """act(norm(x) + residual) and the statistics its backward pass needs."""
+        st = self.store
+        if out is None:
+            out = ctx.empty(tuple(x.shape))
+        mean, rstd = ctx.empty((2, x.shape[0], self.groups), dtype=torch.float32)
+        ops.group_norm_fwd(x, st.view(self.gamma), st.view(self.beta), self.groups, self.eps, out, mean, rstd, act=act,
+                           residual=residual)
+        return out, (mean, rstd)
+
+    def backward(self, ctx: Context, dy, x, stats, dx, act="none", y=None, residual=None, dresidual=None):
+        """dx (may be x or dy), the parameter gradients into the arena, the residual's gradient into dresidual (may be dy)."""
+        st = self.store
+        dg = st.gview(self.gamma) if self.trainable else None
+        db = st.gview(self.beta) if self.trainable else None
+        ops.group_norm_bwd(dy, x, st.view(self.gamma), st.view(self.beta), self.groups, stats[0], stats[1], dx, dg, db, act=act,
+                           y=y, residual=residual, dresidual=dresidual)
+        if self.trainable:
+            ctx.tape.ready(self.gamma)
+            ctx.tape.ready(self.beta)
+        return dx
+
+
+def _gn_act(ctx: Context, gn, z, act, residual, out, needs, dx_out, then):
+    """act(group norm(z) + residual); in the backward pass then(dx), dx written into dx_out()."""
+    out, stats = gn.forward(ctx, z, act, None if residual is None else residual.data, out)
+    y = Act(out, needs)
+    if ctx.grad_enabled and needs:
+        # a ReLU behind a residual is masked by the output; everything else is computed again from z (and the residual)
+        by_y = act == "relu" and residual is not None
+        res = None if residual is None or by_y else residual.data
+
+        def bw():
+            dy = y.grad
+            y.grad = None
+            wants = residual is not None and residual.needs_grad
+            dx = dx_out()
+            gn.backward(ctx, dy, z, stats, dx, act, y=y.data if by_y else None, residual=res, dresidual=dy if wants else None)
+            if wants:
+                accumulate_grad(residual, dy)          # (dy now holds the gradient of the sum under the activation)
+            then(dx)
+        ctx.tape.push(bw)
+    return y
+
+
+class GNAct:
+    """Stand-alone group norm (+ residual) + activation on an arbitrary (possibly channel-sliced) activation."""
+
+    def __init__(self, gn: GroupNorm2d, act="relu"):
+        self.gn, self.act = gn, act
+
+    def __call__(self, ctx: Context, x: Act, residual: Act = None, out=None) -> Act:
+        needs = x.needs_grad or self.gn.trainable or (residual is not None and residual.needs_grad)
+
+        def then(dx):
+            if x.needs_grad:
+                accumulate_grad(x, dx)
+        return _gn_act(ctx, self.gn, x.data, self.act, residual, out, needs, lambda: ctx.empty(tuple(x.data.shape)), then)
+
+
+class ConvGNAct:
+    """conv -> group norm -> (+ residual) -> activation (the place of ConvBNAct in a network without batch statistics)."""
+
+    def __init__(self, conv: Conv2d, gn: GroupNorm2d, act="relu"):
+        self.conv, self.gn, self.act = conv, gn, act
+
+    def __call__(self, ctx: Context, x: Act, relu=True, residual: Act = None, out=None, last_use=False,
+                 defer_apply=False) -> Act:
+        """relu=False: no activation; defer_apply is ConvBNAct's (a group norm is never left to its consumer)."""
+        conv = self.conv
+        z = conv.forward_raw(ctx, x.data)
+        needs = x.needs_grad or conv.trainable or self.gn.trainable or (residual is not None and residual.needs_grad)
+        # dx overwrites z (dead after this)
+        return _gn_act(ctx, self.gn, z, self.act if relu else "none", residual, out, needs, lambda: z,
+                       lambda dx: conv.backward_raw(ctx, x, dx, last_use=last_use))
+
+
 class Linear(Conv2d):
     """nn.Linear as a convolution: [N,1,1,in] x 1x1, or (after a spatial map) [N,H,W,C] x (H x W) 'valid'."""
 
@@ -631,6 +720,77 @@ class Linear(Conv2d):
             c, h, w = spatial
             assert c * h * w == in_features
             super().__init__(store, name, c, out_features, (h, w), linear=True, **kw)
+
+
+class Mlp:
+    """Chain of linear products over [N, 1, 1, C]: x -> act(x W0^T + b0) -> ... -> x Wn^T + bn (+ residual).  Bias, activation
+    and residual are epilogues of the products; in the backward pass a product's data gradient comes out multiplied by the
+    derivative of the activation before it, and the weight and bias gradients go straight into the arena.  Parameters are
+    named like torch's Sequential of Linear and activation modules (name.0, name.2, ...), or `name` for a single product."""
+
+    def __init__(self, store: ParamStore, name, widths, act="gelu", trainable=True):
+        self.store, self.act, self.trainable, n = store, act, trainable, len(widths) - 1
+        if n < 1:
+            raise ValueError(f"{name}: an MLP has an input and an output width, got {tuple(widths)}")
+        self.layers = []
+        for i, (cin, cout) in enumerate(zip(widths, widths[1:])):
+            at = name if n == 1 else f"{name}.{2 * i}"
+            self.layers.append((store.add_conv_weight(f"{at}.weight", cout, cin, 1, 1, kaiming_uniform_default, trainable,
+                                                      flat_logical=True),
+                                store.add_vec(f"{at}.bias", cout, bias_default(cin), trainable)))
+
+    def _w(self, spec):
+        w = self.store.cview(spec)
+        return w.view(w.shape[0], -1)
+
+    def __call__(self, ctx: Context, x: Act, residual: Act = None) -> Act:
+        st = self.store
+        n = x.data.shape[0]
+        if tuple(x.data.shape) != (n, 1, 1, x.data.shape[3]):
+            raise ValueError(f"an MLP takes [N, 1, 1, C], got {tuple(x.data.shape)}")
+        needs = x.needs_grad or self.trainable or (residual is not None and residual.needs_grad)
+        track = ctx.grad_enabled and needs
+        h, kept = x.data.view(n, -1), []          # (input, pre-activation) of every product
+        for i, (ws, bs) in enumerate(self.layers):
+            w, last = self._w(ws), i == len(self.layers) - 1
+            y = ctx.empty((n, w.shape[0]))
+            z = ctx.empty((n, w.shape[0])) if track and not last and self.act != "none" else None
+            ops.linear_fprop(h, w, y, st.view(bs), act="none" if last else self.act,
+                             addend=residual.data.view(n, -1) if last and residual is not None else None, preact=z)
+            kept.append((h, z))
+            h = y
+        y = Act(h.view(n, 1, 1, -1), needs)
+        if track:
+            def bw():
+                top = y.grad
+                y.grad = None
+                dy = top.view(n, -1)
+                for i in reversed(range(len(self.layers))):
+                    (ws, bs), (h, _) = self.layers[i], kept[i]
+                    if self.trainable:
+                        gw = st.gview(ws)
+                        ops.linear_wgrad(dy, h, gw.view(gw.shape[0], -1), st.gview(bs))
+                        ctx.tape.ready(bs)
+                        ctx.tape.ready(ws)
+                    if i > 0:
+                        dh = ctx.empty(tuple(h.shape))
+                        z = kept[i - 1][1]
+                        ops.linear_dgrad(dy, self._w(ws), dh, act="none" if z is None else self.act, preact=z)
+                        dy = dh
+                    elif x.needs_grad:
+                        if residual is x:
+                            accumulate_grad(x, top)
+                        add = None if x.grad is None else x.grad.view(n, -1)
+                        g = x.grad if add is not None else x.grad_buf
+                        if g is None or g.data_ptr() == dy.data_ptr():          # (a product may not overwrite its operand)
+                            g = ctx.empty(tuple(x.data.shape))
+                        ops.linear_dgrad(dy, self._w(ws), g.view(n, -1), addend=add)
+                        x.grad = g
+                if residual is not None and residual is not x and residual.needs_grad:
+                    accumulate_grad(residual, top)
+                kept.clear()
+            ctx.tape.push(bw)
+        return y
 
 
 # ------------------------------------------------------------------------------------------------ pooling etc.

@@ -4,13 +4,19 @@ DDP bucket so the update of bucket k overlaps the all-reduce of bucket k+1).  lr
 vector so a captured hipGraph stays valid when they change.  `state_dict()` reproduces torch.optim's layout
 (per-parameter `step` 0-d fp32 tensor, `exp_avg`, `exp_avg_sq` / `momentum_buffer`) in torchvision's
 OIHW layout so the reference's `optimizer.load_state_dict` accepts it.
+
+"adamw" decouples the weight decay and applies it to matrices and filters only: biases and norm scales are a parameter group
+of their own, without decay, and `state_dict()` has the layout of torch.optim.AdamW over those two groups (decayed parameters
+first).  "adamw8" is the same with states of 8 bits (ops.adamw8_step): 2.03 bytes a parameter instead of 8.  It is saved as the
+32-bit values its states stand for, with the scales as entries of the first parameter group; loading rounds to nearest,
+which gives the same codes again.  A checkpoint of one kind loads into the other.
 """
 from __future__ import annotations
 
 import torch
 
 from .. import ops
-from .engine import ParamStore
+from .engine import ALIGN, ParamStore, pad_to
 
 # hyper vector slots (csrc/hip/optim.hip)
 LR, B1, B2, EPS, WD, STEP, MOM, GSCALE, OMB1, OMB2, B1LO, B2LO = range(12)
@@ -29,16 +35,36 @@ def make_hyper(lr, beta1, beta2, eps, weight_decay, step, momentum, grad_scale, 
 
 
 class ArenaOptimizer:
-    def __init__(self, store: ParamStore, kind="adam", lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
-                 momentum=0.9, grad_scale=1.0):
-        if kind not in ("adam", "SGD"):
+    def __init__(self, store: ParamStore, kind="adam", lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=None,
+                 momentum=0.9, grad_scale=1.0, seed=0):
+        """weight_decay: 0.01 for "adamw" and "adamw8", 0 for the others where it is not given.  seed: of the stochastic rounding
+        of 8-bit states; ranks that share a model must share it."""
+        if kind not in ("adam", "SGD", "adamw", "adamw8"):
             raise ValueError(f"Invalid optimizer {kind!r}")
         self.store, self.kind = store, kind
+        self.adamw = kind in ("adamw", "adamw8")
+        if weight_decay is None:
+            weight_decay = 0.01 if self.adamw else 0.0
         dev = store.device
         self.hyper = make_hyper(lr, betas[0], betas[1], eps, weight_decay, 0.0, momentum if kind == "SGD" else 0.0,
                                 grad_scale, device=dev)
-        self.m = torch.zeros_like(store.p)
-        self.v = torch.zeros_like(store.p) if kind == "adam" else None
+        self.m_scale = self.v_scale = self.groups = self.group_ids = None
+        self.seed = int(seed) & 0xFFFFFFFF
+        if kind == "adamw8":
+            n = store.p.numel()
+            self.m = torch.zeros(n, dtype=torch.float8_e4m3fn, device=dev)
+            self.v = torch.zeros(n, dtype=torch.float8_e5m2, device=dev)
+            self.m_scale, self.v_scale = torch.zeros(n // ALIGN, device=dev), torch.zeros(n // ALIGN, device=dev)
+        else:
+            self.m = torch.zeros_like(store.p)
+            self.v = torch.zeros_like(store.p) if kind != "SGD" else None
+        if self.adamw:
+            ids = torch.zeros(store.p.numel() // ALIGN, dtype=torch.uint8)
+            for spec in store.params:
+                if spec.kind == "vec":
+                    ids[spec.offset // ALIGN: (spec.offset + pad_to(spec.numel, ALIGN)) // ALIGN] = 1
+            self.group_ids = ids.to(dev)
+            self.groups = torch.tensor([[1.0, 1.0], [1.0, 0.0]], device=dev)
         self.defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, momentum=momentum)
         self.base_lr = lr
         self._host_step = 0
@@ -49,6 +75,11 @@ class ArenaOptimizer:
         s = self.store
         if self.kind == "adam":
             ops.adam_step(s.p, s.g, self.m, self.v, s.p16, self.hyper, lo, hi)
+        elif self.kind == "adamw":
+            ops.adamw_step(s.p, s.g, self.m, self.v, s.p16, self.hyper, self.groups, self.group_ids, lo, hi)
+        elif self.kind == "adamw8":
+            ops.adamw8_step(s.p, s.g, self.m, self.v, self.m_scale, self.v_scale, s.p16, self.hyper, self.groups, self.group_ids,
+                            self.seed, lo, hi)
         else:
             ops.sgd_step(s.p, s.g, self.m, s.p16, self.hyper, lo, hi)
 
@@ -60,6 +91,10 @@ class ArenaOptimizer:
         for lo, hi in self.store.trainable_ranges():
             self.step_range(lo, hi)
         self.finish_step()
+
+    def state_tensors(self):
+        """Everything a step changes beside the parameters: what a capture's warm-up has to put back."""
+        return [t for t in (self.m, self.v, self.m_scale, self.v_scale, self.hyper) if t is not None]
 
     def set_lr(self, lr):
         self._host_lr = lr
@@ -79,49 +114,91 @@ class ArenaOptimizer:
         st = self.store
         state = {}
         step = float(self.hyper[STEP].item())
+        order = self._order()
         if step > 0:
-            for i, spec in enumerate(st.params):
+            for i, spec in enumerate(order):
                 if not spec.trainable:
                     continue
-                sl = slice(spec.offset, spec.offset + spec.numel)
-                if self.kind == "adam":
-                    state[i] = {"step": torch.tensor(step, dtype=torch.float32),
-                                "exp_avg": st.storage_to_logical(spec, self.m[sl].view(spec.storage_shape)),
-                                "exp_avg_sq": st.storage_to_logical(spec, self.v[sl].view(spec.storage_shape))}
+                m, v = self._moments(spec)
+                if self.kind != "SGD":
+                    state[i] = {"step": torch.tensor(step, dtype=torch.float32), "exp_avg": st.storage_to_logical(spec, m),
+                                "exp_avg_sq": st.storage_to_logical(spec, v)}
                 else:
-                    state[i] = {"momentum_buffer": st.storage_to_logical(spec, self.m[sl].view(spec.storage_shape))}
+                    state[i] = {"momentum_buffer": st.storage_to_logical(spec, m)}
         lr = float(self.get_lr())
-        if self.kind == "adam":
+        if self.kind != "SGD":
             group = {"lr": lr, "betas": tuple(self.defaults["betas"]), "eps": self.defaults["eps"],
                      "weight_decay": self.defaults["weight_decay"], "amsgrad": False, "maximize": False, "foreach": None,
-                     "capturable": False, "differentiable": False, "fused": None, "decoupled_weight_decay": False}
+                     "capturable": False, "differentiable": False, "fused": None, "decoupled_weight_decay": self.adamw}
         else:
             group = {"lr": lr, "momentum": self.defaults["momentum"], "dampening": 0, "weight_decay":
                      self.defaults["weight_decay"], "nesterov": False, "maximize": False, "foreach": None,
                      "differentiable": False, "fused": None, "initial_lr": self.base_lr}
-        group["params"] = list(range(len(st.params)))
-        return {"state": state, "param_groups": [group]}
+        groups = [dict(group, params=list(range(len(order))))]
+        if self.adamw:
+            k = sum(spec.kind != "vec" for spec in order)
+            groups = [dict(group, params=list(range(k))), dict(group, weight_decay=0.0, params=list(range(k, len(order))))]
+        if self.kind == "adamw8" and step > 0:
+            groups[0].update(m_scale=self.m_scale.clone(), v_scale=self.v_scale.clone())
+        return {"state": state, "param_groups": groups}
+
+    def _order(self):
+        """The parameters as torch numbers them: in registration order, group by group."""
+        ps = self.store.params
+        return [s for s in ps if s.kind != "vec"] + [s for s in ps if s.kind == "vec"] if self.adamw else ps
+
+    def _moments(self, spec):
+        """(exp_avg or momentum, exp_avg_sq or None) of a parameter, fp32, in storage layout."""
+        sl = slice(spec.offset, spec.offset + spec.numel)
+        if self.kind != "adamw8":
+            return self.m[sl].view(spec.storage_shape), None if self.v is None else self.v[sl].view(spec.storage_shape)
+        lo, hi = spec.offset, spec.offset + pad_to(spec.numel, ALIGN)
+        b = slice(lo // ALIGN, hi // ALIGN)
+        return tuple(ops.adamw8_decode(t[lo:hi], s[b])[: spec.numel].view(spec.storage_shape)
+                     for t, s in ((self.m, self.m_scale), (self.v, self.v_scale)))
+
+    def _set_moment(self, spec, which, logical):
+        st = self.store
+        logical = logical.to(st.device, torch.float32)
+        t = self.m if which == "m" else self.v
+        if self.kind != "adamw8":
+            st.logical_to_storage(spec, logical, t[spec.offset: spec.offset + spec.numel].view(spec.storage_shape))
+            return
+        lo, hi = spec.offset, spec.offset + pad_to(spec.numel, ALIGN)
+        full = torch.zeros(hi - lo, device=st.device)
+        st.logical_to_storage(spec, logical, full[: spec.numel].view(spec.storage_shape))
+        codes, scales = ops.adamw8_encode(full, torch.full_like(full, 0.5), which)
+        t[lo:hi] = codes
+        (self.m_scale if which == "m" else self.v_scale)[lo // ALIGN: hi // ALIGN] = scales
 
     def load_state_dict(self, sd):
         st = self.store
-        group = sd["param_groups"][0]
-        if len(group["params"]) != len(st.params):
-            raise ValueError(f"optimizer state_dict covers {len(group['params'])} parameters, the model has "
-                             f"{len(st.params)}")
-        self.set_lr(float(group["lr"]))
+        groups, order = sd["param_groups"], self._order()
+        have = [len(g["params"]) for g in groups]
+        k = sum(spec.kind != "vec" for spec in order)
+        want = [k, len(order) - k] if self.adamw else [len(order)]
+        if have != want:
+            raise ValueError(f"optimizer state_dict covers {sum(have)} parameters in groups of {have}, the model has "
+                             f"{len(st.params)} in groups of {want}" if self.adamw or len(have) > 1 else
+                             f"optimizer state_dict covers {have[0]} parameters, the model has {len(st.params)}")
+        self.set_lr(float(groups[0]["lr"]))
         step = 0.0
-        for i, spec in enumerate(st.params):
+        for i, spec in enumerate(order):
             s = sd["state"].get(i)
             if s is None or not spec.trainable:
                 continue
-            sl = slice(spec.offset, spec.offset + spec.numel)
-            if self.kind == "adam":
+            if self.kind != "SGD":
                 step = float(s["step"])
-                st.logical_to_storage(spec, s["exp_avg"].to(st.device, torch.float32), self.m[sl].view(spec.storage_shape))
-                st.logical_to_storage(spec, s["exp_avg_sq"].to(st.device, torch.float32), self.v[sl].view(spec.storage_shape))
+                self._set_moment(spec, "m", s["exp_avg"])
+                self._set_moment(spec, "v", s["exp_avg_sq"])
             else:
                 step = max(step, 1.0)
-                st.logical_to_storage(spec, s["momentum_buffer"].to(st.device, torch.float32), self.m[sl].view(spec.storage_shape))
+                self._set_moment(spec, "m", s["momentum_buffer"])
+        for key, mine in (("m_scale", self.m_scale), ("v_scale", self.v_scale)):
+            if mine is not None and torch.is_tensor(groups[0].get(key)):
+                if groups[0][key].numel() != mine.numel():
+                    raise ValueError(f"optimizer state_dict holds {groups[0][key].numel()} scales, the model has {mine.numel()}")
+                mine.copy_(groups[0][key])          # (a code times its scale, rounded, may give a scale half a step away)
         self.hyper[STEP] = step
         self._host_step = int(step)
 

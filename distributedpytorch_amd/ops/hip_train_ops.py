@@ -310,7 +310,7 @@ def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
     ap, ag, a16, ah, agr, aid, am, av = at
     b = 4 * lo
     _run(p.device, lambda stream: _lib().dpa_adamw_step(VP(ap + b), VP(ag + b), VP(am + b), VP(av + b), VP(a16 and a16 + 2 * lo), VP(ah), VP(agr),
-                                                        VP(aid + lo // 64), I64(hi - lo), stream))
+                                                        groups.shape[0], VP(aid + lo // 64), I64(hi - lo), stream))
 
 
 def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, seed, lo=0, hi=None):
@@ -321,5 +321,5 @@ def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, see
     ap, ag, a16, ah, agr, aid, am, av, ams, avs = at
     b, s = 4 * lo, lo // 16
     _run(p.device, lambda stream: _lib().dpa_adamw8_step(VP(ap + b), VP(ag + b), VP(am + lo), VP(av + lo), VP(ams + s), VP(avs + s),
-                                                         VP(a16 and a16 + 2 * lo), VP(ah), VP(agr), VP(aid + lo // 64),
+                                                         VP(a16 and a16 + 2 * lo), VP(ah), VP(agr), groups.shape[0], VP(aid + lo // 64),
                                                          ctypes.c_uint(seed & 0xFFFFFFFF), I64(lo), I64(hi - lo), stream))

@@ -641,7 +641,7 @@ def _adamw_update(p, g, m, v, p16, hyper, groups, group_ids, lo, hi):
     h = [float(x) for x in hyper]
     lr, b1, b2, eps, wd, step, _, gs, omb1, omb2 = h[:10]
     b1d, b2d = b1 + h[10], b2 + h[11]
-    per = groups[group_ids[lo // 64: hi // 64].long()].repeat_interleave(64, 0)
+    per = groups[group_ids[lo // 64: hi // 64].long().clamp_max(groups.shape[0] - 1)].repeat_interleave(64, 0)
     gr = g[lo:hi] * gs
     m = m + omb1 * (gr - m)
     v = b2 * v + omb2 * gr * gr
@@ -657,7 +657,7 @@ def _adamw_update(p, g, m, v, p16, hyper, groups, group_ids, lo, hi):
 def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
     """AdamW (decay decoupled from the gradient) on the range [lo, hi) of an arena whose tensors start at multiples of 64
     elements.  hyper: nn/optim.py make_hyper, whose lr and weight decay are multiplied by the two entries of
-    groups[group_ids[i]] (fp32 [rows, 2]; uint8, one for each 64 elements).  p16: the bf16 compute copy, or None."""
+    groups[group_ids[i]] (fp32 [rows, 2]; uint8, one for each 64 elements; ids beyond the rows take the last one).  p16: the bf16 compute copy, or None."""
     from . import checks
     n = p.numel()
     hi, _ = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi, (("m", m, torch.float32, n), ("v", v, torch.float32, n)))

@@ -146,9 +146,7 @@ class DistributedModel:
         self._static_x, self._static_y = x.clone(), labels.clone()
         # warm-up iterations must not perturb training: snapshot every piece of mutable state and restore it
         st, opt = self.net.store, self.opt
-        state = [st.p, st.buffer_arena, opt.m, opt.hyper, self.net.rng, self.accum, self.metrics]
-        if opt.v is not None:
-            state.append(opt.v)
+        state = [st.p, st.buffer_arena, *opt.state_tensors(), self.net.rng, self.accum, self.metrics]
         if st.p16 is not None:
             state.append(st.p16)
         state.extend(st.aux_tensors)       # BatchNorm's statistics shift (previous batch mean) is carried state too

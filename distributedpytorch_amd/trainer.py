@@ -53,6 +53,13 @@ def _dtype(cfg, device):
     return torch.bfloat16 if getattr(cfg, "COMPUTE_DTYPE", "fp32") == "bf16" else torch.float32
 
 
+def _model_options(cfg):
+    """Norm, activation and classifier of the networks that have a choice (models/factory.py)."""
+    kw = dict(norm=getattr(cfg, "NORM", "batch"), act=getattr(cfg, "ACT", "relu"),
+              head_hidden=tuple(int(w) for w in str(getattr(cfg, "HEAD_HIDDEN", "")).split(",") if w.strip()))
+    return kw if kw != dict(norm="batch", act="relu", head_hidden=()) else {}
+
+
 def _maybe_fault(cfg, rank, step):
     spec = getattr(cfg, "FAULT_INJECT", "")
     if spec:
@@ -133,7 +140,8 @@ def _build(args, gpu, rank, modelName, cfg, with_optimizer):
     dataset = MNIST(args.dataPath, args.batchSize, get_model_input_size(modelName), worldSize=args.worldSize, rank=rank,
                     gpu=gpu, device=device, dtype=dtype, debug=bool(args.debug), seed=cfg.SEED,
                     synthetic_ok=getattr(cfg, "SYNTHETIC_DATA", False))
-    net, _ = get_model(modelName, dataset.nbClasses, cfg.FEATURE_EXTRACT, cfg.USE_PRETRAINED, device=device, dtype=dtype)
+    net, _ = get_model(modelName, dataset.nbClasses, cfg.FEATURE_EXTRACT, cfg.USE_PRETRAINED, device=device, dtype=dtype,
+                       **_model_options(cfg))
     net.seed_rng(cfg.SEED)
     loss_kind = cfg.LOSS if with_optimizer else "cross_entropy"
     if loss_kind == "cross_entropy":
@@ -150,6 +158,8 @@ def _build(args, gpu, rank, modelName, cfg, with_optimizer):
             optimizer = ArenaOptimizer(net.store, "adam", lr=0.001)
         elif cfg.OPTIMIZER == "SGD":
             optimizer = ArenaOptimizer(net.store, "SGD", lr=0.001, momentum=0.9)
+        elif cfg.OPTIMIZER in ("adamw", "adamw8"):
+            optimizer = ArenaOptimizer(net.store, cfg.OPTIMIZER, lr=0.001, weight_decay=getattr(cfg, "WEIGHT_DECAY", 0.01), seed=cfg.SEED)
         else:
             logging.error("Invalid optimizer, exiting...")
             raise SystemExit(1)
