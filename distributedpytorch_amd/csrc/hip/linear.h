@@ -21,8 +21,9 @@ struct LinParams {
   const void *addend, *pre;             // pre: z of the activation whose derivative is multiplied in
   void *out, *preact;
   float* ws;                            // [splits][rows][cols] partial products where splits > 1
+  float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns: the bias gradient), or null
   long long ld_add, ld_pre, ld_out, ld_z;
-  int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, pad;      // vec: every matrix of the epilogue takes 16-byte access
+  int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
 };
 
 // What a call hands over besides: the operands as they are, what they are packed into first (ld 0: nothing), the bias gradient.
@@ -172,6 +173,9 @@ __device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int
 // all but this wave's newest N pieces have landed and its LDS reads are done; behind the barrier, everyone's
 template <int N> __device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
+// a kernel that can make the row sums on its way (the 256 x 256 tile has no registers for them, fp32 has three parts)
+template <int MT, int P, int EPI> constexpr bool lin_sums() { return EPI == EPI_WGRAD && P == 1 && MT <= 4; }
+
 // The blocks are persistent and see ONE stream of K steps across their tiles, S of them in LDS: while step s is multiplied, the
 // steps behind it land, and step s + S is requested as soon as the buffer of step s is free, also when it belongs to the next
 // tile, so the epilogue of a tile runs under the first loads of the next.
@@ -290,6 +294,15 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
           for (int j = 0; j < NT; ++j) mfma(fb[ks][j], fa[half * H + i], acc[half * H + i][j]);
       };
+      // Sums of a's rows on the matrix pipe: a times a fragment whose column i is ones adds row tile i to column i of one
+      // accumulator.  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
+      // 2 MT of them in a step of `takers`.  8192 x 4096 x 1024 with the bias gradient: 99 us, with a pass of its own over dy
+      // 110, without 95.
+      constexpr bool SUMS = lin_sums<MT, P, EPI>();
+      f32x4 sums = {0.f, 0.f, 0.f, 0.f};
+      const int taker = j0 / BN * WN + wn;
+      const bool takes = SUMS && p.sums && taker < p.takers;
+      int turn = takes ? taker : 0x7fffffff;
       read_b(0);
       read_a(0, 0);
       for (; steps > 0; --steps) {
@@ -302,6 +315,18 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         __builtin_amdgcn_sched_barrier(0);
         read_a(1, 1);
         multiply(0, 1);
+        if constexpr (SUMS) {
+          if (--turn < 0) {          // (one branch a step, and fragments of its own: the steps without it lose nothing)
+            turn = p.takers - 1;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                const short one = (lane & 15) == i ? (short)0x3F80 : (short)0;
+                sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_at(buf, 0, i, ks), (bf16x8)one, sums, 0, 0, 0);
+              }
+          }
+        }
         lin_sync<(S - 2) * PP>();
         buf = buf + 1 == S ? 0 : buf + 1;
         if (steps > 1) {
@@ -317,6 +342,12 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         }
         requested();
         __builtin_amdgcn_sched_barrier(0);
+      }
+      if (takes && (lane & 15) < MT) {
+        const int r0 = i0 + (wm * MT + (lane & 15)) * 16 + (lane >> 4) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (r0 + e < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + r0 + e] = sums[e];
       }
     } else {
       struct Parts { bf16x8 a[P][MT], b[P][NT]; } even, odd;

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) lin_pack_kernel(LinPack one, LinPack two)
   }
 }
 
-// ---- bias gradient: column sums of dy [M, N] in two steps, S row ranges into a slab [S, N], then the slab in a fixed order.
+// ---- bias gradient where the product does not make it (lin_sums): column sums of dy [M, N] in two steps, S row ranges into a slab [S, N], then the slab in a fixed order.
 // A lane owns one 16-byte vector of columns (VEC) or one column and keeps eight rows in flight; `lanes` lanes side by side.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) lin_colsum_kernel(const T* __restrict__ x, long long ld, int rows, int cols, int per, int lanes, float* __restrict__ slab) {
@@ -227,6 +227,7 @@ DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
     case EPI_WGRAD: rc = lin_wgrad(c.p, c.tile, s); break;
   }
   if (rc || !c.db) return rc;
-  if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
+  if (c.p.sums) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.db_splits, c.a_cols, c.p.accumulate, c.db);
+  else if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
   return dpa_launch_rc();
 }

@@ -28,9 +28,9 @@ class GnParams(ctypes.Structure):
 
 class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
     _fields_ = [("a", VP), ("b", VP), ("lda", I64), ("ldb", I64), ("a_part", I64), ("b_part", I64), ("bias", VP), ("addend", VP), ("pre", VP),
-                ("out", VP), ("preact", VP), ("ws", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
+                ("out", VP), ("preact", VP), ("ws", VP), ("sums", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
                 ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("vec", I32),
-                ("bias_vec", I32), ("pad", I32),
+                ("bias_vec", I32), ("takers", I32),
                 ("src_a", VP), ("src_b", VP), ("pack_a", VP), ("pack_b", VP), ("db", VP), ("db_slab", VP), ("src_lda", I64), ("src_ldb", I64),
                 ("a_rows", I32), ("a_cols", I32), ("b_rows", I32), ("b_cols", I32), ("ld_a", I32), ("ld_b", I32), ("vec_a", I32), ("vec_b", I32),
                 ("db_splits", I32), ("epi", I32), ("tile", I32), ("f32", I32)]
@@ -196,7 +196,7 @@ def _plan(rows, cols, k, f32):
     return 3, max(1, min(512 // t64, k // 512, 16))
 
 
-def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
+def _linear(stream, c, t_a, a, t_b, b, k, device):
     """Fills in the operands, the plan and the workspace of a call whose epilogue is set, and launches it."""
     c.src_a, c.src_lda, _ = a
     c.src_b, c.src_ldb, _ = b
@@ -228,7 +228,13 @@ def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
             steps = _cdiv(k, 32 if c.tile >= 4 else 64) * (6 if f32 and c.tile < 4 else 1)
             c.splits = _cdiv(steps, _cdiv(steps, c.splits))          # no range is empty
             need += c.splits * c.rows * c.cols * 4 + 15 & ~15
-    need += db_slab * 4
+        if c.db:          # (an fprop has none)
+            if not f32 and c.tile > 0:          # the product makes the sums: 2 waves in each of the tiles of a row
+                c.takers = min(2 * _cdiv(c.cols, 64 if c.tile == 3 else 128), 16)
+                c.db_splits = c.splits * c.takers
+            else:
+                c.db_splits = max(1, min(_cdiv(k, 32), 1024 // _cdiv(c.rows, 512)))
+            need += c.db_splits * c.rows * 4
     if need:
         ws = torch.empty(need, device=device, dtype=torch.uint8)
         at = ws.data_ptr()
@@ -241,7 +247,10 @@ def _linear(stream, c, t_a, a, t_b, b, k, device, db_slab):
         if c.splits > 1:
             c.ws = at
             at += c.splits * c.rows * c.cols * 4 + 15 & ~15
-        c.db_slab = at
+        if c.takers:
+            c.sums = at
+        else:
+            c.db_slab = at
     _lib().dpa_linear(byref(c), stream)
 
 
@@ -259,7 +268,7 @@ def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
     f32 = c.f32 = x.dtype is _F32
     c.vec = not (n & 7 or (ys[0] | ads[0] | zs[0] | (ys[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
     c.bias_vec = not (n & 7 or b & 15)
-    _run(x.device, _linear, c, x, xs, w, ws, k, x.device, 0)
+    _run(x.device, _linear, c, x, xs, w, ws, k, x.device)
     return y
 
 
@@ -276,7 +285,7 @@ def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
     c.addend, c.ld_add, _ = ads
     f32 = c.f32 = dy.dtype is _F32
     c.vec = not (k & 7 or (dxs[0] | ads[0] | zs[0] | (dxs[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
-    _run(dy.device, _linear, c, dy, dys, w, ws, n, dy.device, 0)
+    _run(dy.device, _linear, c, dy, dys, w, ws, n, dy.device)
     return dx
 
 
@@ -295,11 +304,7 @@ def linear_wgrad(dy, x, dw, db=None, accumulate=False):
     c.out, c.ld_out, _ = dws
     c.f32 = dy.dtype is _F32
     c.vec = not (k & 7 or (dws[0] | dws[1] * 4) & 15)
-    slab = 0
-    if b:
-        c.db_splits = max(1, min(_cdiv(m, 32), 1024 // _cdiv(n, 512)))
-        slab = c.db_splits * n
-    _run(dy.device, _linear, c, dy, dys, x, xs, m, dy.device, slab)
+    _run(dy.device, _linear, c, dy, dys, x, xs, m, dy.device)
     return dw
 
 
