@@ -294,12 +294,14 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
           for (int j = 0; j < NT; ++j) mfma(fb[ks][j], fa[half * H + i], acc[half * H + i][j]);
       };
-      // Sums of a's rows on the matrix pipe: a times a fragment whose column i is ones adds row tile i to column i of one
-      // accumulator.  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
+      // Sums of a's rows on the matrix pipe: a times ones, an accumulator for each row tile (one for all, with ones in a column
+      // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
       // 2 MT of them in a step of `takers`.  8192 x 4096 x 1024 with the bias gradient: 99 us, with a pass of its own over dy
       // 110, without 95.
       constexpr bool SUMS = lin_sums<MT, P, EPI>();
-      f32x4 sums = {0.f, 0.f, 0.f, 0.f};
+      f32x4 sums[SUMS ? MT : 1];
+#pragma unroll
+      for (int i = 0; i < (SUMS ? MT : 1); ++i) sums[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
       const int taker = j0 / BN * WN + wn;
       const bool takes = SUMS && p.sums && taker < p.takers;
       int turn = takes ? taker : 0x7fffffff;
@@ -321,10 +323,8 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                const short one = (lane & 15) == i ? (short)0x3F80 : (short)0;
-                sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_at(buf, 0, i, ks), (bf16x8)one, sums, 0, 0, 0);
-              }
+              for (int i = 0; i < MT; ++i)
+                sums[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_at(buf, 0, i, ks), (bf16x8)(short)0x3F80, sums[i], 0, 0, 0);
           }
         }
         lin_sync<(S - 2) * PP>();
@@ -343,11 +343,16 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         requested();
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (takes && (lane & 15) < MT) {
-        const int r0 = i0 + (wm * MT + (lane & 15)) * 16 + (lane >> 4) * 4;
+      if constexpr (SUMS) {
+        if (takes && (lane & 15) == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (r0 + e < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + r0 + e] = sums[e];
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int row = i0 + (wm * MT + i) * 16 + (lane >> 4) * 4 + e;
+              if (row < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + row] = sums[i][e];
+            }
+        }
       }
     } else {
       struct Parts { bf16x8 a[P][MT], b[P][NT]; } even, odd;

@@ -176,6 +176,32 @@ def test_a_bad_value_stays_in_its_group(dtype, hw, c, act):
             assert torch.equal(a.permute(0, 2, 1, 3)[rest], b.permute(0, 2, 1, 3)[rest])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("m,n,k", [(70, 130, 72), (300, 260, 264), (1000, 520, 4100)], ids=str)
+def test_a_bad_value_stays_in_its_row(dtype, m, n, k):
+    """A NaN in one row of x or one column of dy reaches that row of y and dx, that row of dw and that entry of db, and nothing else."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w, dy = (torch.randn(*s, device="cuda", generator=g).to(dtype) for s in ((m, k), (n, k), (m, n)))
+    bias = torch.randn(n, device="cuda", generator=g)
+
+    def run(x, dy):
+        y, dx, dw, db = torch.empty(m, n, device="cuda", dtype=dtype), torch.empty_like(x), torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+        ops.linear_fprop(x, w, y, bias, act="gelu")
+        ops.linear_dgrad(dy, w, dx)
+        ops.linear_wgrad(dy, x, dw, db)
+        return y, dx, dw, db
+    want = run(x, dy)
+    for value in (float("nan"), float("inf")):
+        xb, dyb = x.clone(), dy.clone()
+        xb[5, 3], dyb[7, 37] = value, value
+        y, _, dwx, _ = run(xb, dy)
+        _, dx, dw, db = run(x, dyb)
+        rows, cols, outs = (torch.arange(s, device="cuda") for s in (m, k, n))
+        for got, ref, rest in ((y, want[0], rows != 5), (dx, want[1], rows != 7), (dw, want[2], outs != 37), (db, want[3], outs != 37)):
+            assert torch.equal(got[rest], ref[rest]) and not torch.isfinite(got[~rest]).all()
+        assert torch.equal(dwx[:, cols != 3], want[2][:, cols != 3]) and not torch.isfinite(dwx[:, 3]).any()
+
+
 def test_group_norm_beyond_31_bits_of_elements():
     """A channel slice of a wide buffer whose last image starts behind 2^31 elements, against that image alone."""
     n, h, w, c, wide = 5, 640, 512, 16, 1704
