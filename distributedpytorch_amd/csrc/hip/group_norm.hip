@@ -19,7 +19,7 @@ struct GnParams {
   int act, W, rows, R, threads, way;    // the vector kernels: vectors of a chunk, pixels of a sweep, sweeps, threads, which kernel
   float eps;
 };
-enum : int { GN_ANY = 0, GN_ONE = 1, GN_TWO = 2 };
+enum : int { GN_ANY = 0, GN_ONE = 1, GN_TWO = 2, GN_LONE = 3 };      // GN_LONE: one pass, one channel a lane
 
 __device__ __forceinline__ int gn_count(const GnParams& p, int s) { return min(p.pps, p.HW - s * p.pps); }
 
@@ -140,25 +140,32 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(GnParams p) {
 }
 
 // one wave per (image, group): c1, c2
-__global__ void __launch_bounds__(64) gn_bwd_coef_kernel(GnParams p) {
+__device__ __forceinline__ void gn_bwd_coef(const GnParams& p, long long first, long long step) {
+  const int lane = threadIdx.x & 63;
   const float inv = 1.f / ((float)p.HW * (float)p.cg);
-  for (long long q = blockIdx.x; q < (long long)p.N * p.G; q += gridDim.x) {
+  for (long long q = first; q < (long long)p.N * p.G; q += step) {
     const int n = (int)(q / p.G), g = (int)(q % p.G), total = p.S * p.cg;
     const float* o = p.slab + (long long)n * p.S * 2 * p.C + g * p.cg;
     float sa = 0.f, sb = 0.f;
-    for (int i = threadIdx.x; i < total; i += 64) {
+#pragma unroll 2
+    for (int i = lane; i < total; i += 64) {
       const int s = i / p.cg, k = i - s * p.cg;
       const float* e = o + (long long)s * 2 * p.C + k;
       const float gm = p.gamma[g * p.cg + k];
       sa += e[0] * gm; sb += e[p.C] * gm;
     }
     sa = wave_sum(sa); sb = wave_sum(sb);
-    if (threadIdx.x == 0) { p.coef[2 * q] = sa * inv; p.coef[2 * q + 1] = sb * inv; }
+    if (lane == 0) { p.coef[2 * q] = sa * inv; p.coef[2 * q + 1] = sb * inv; }
   }
 }
 
-// dgamma / dbeta: 16 channels x 64 row lanes over the N * S rows of the slab, in a fixed order
-__global__ void __launch_bounds__(1024) gn_bwd_params_kernel(GnParams p) {
+// dgamma / dbeta in the first `strips` blocks: 16 channels x 64 row lanes over the N * S rows of the slab, in a fixed order.  The
+// blocks behind them make the coefficients of dx where it has a kernel of its own for any layout: one launch for both.
+__global__ void __launch_bounds__(1024) gn_bwd_params_kernel(GnParams p, int strips) {
+  if ((int)blockIdx.x >= strips) {
+    gn_bwd_coef(p, (long long)(blockIdx.x - strips) * 16 + (threadIdx.x >> 6), (long long)(gridDim.x - strips) * 16);
+    return;
+  }
   __shared__ float sh[2][64][17];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
   const int rows = p.N * p.S;
@@ -213,6 +220,22 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(GnParams p) {
 // a vector, some 25 instructions an element, is the next bound, so sign and branch decisions are made once a vector.  Sums over
 // the lanes of a wave stay in registers (DPP and lane swaps): through LDS 28 x 28 x 512 backward took 84 us.
 
+// What a thread holds of a pixel: 16 bytes, or one channel (Lone<T>) where the layout allows no more.
+template <typename T> struct Lone;
+template <typename T> struct GnTypes { typedef T E; typedef Vec16<T> X; };
+template <typename T> struct GnTypes<Lone<T>> {
+  typedef T E;
+  struct X {
+    static constexpr int N = 1;
+    float v;
+    __device__ __forceinline__ void load(const T* p) { v = Elem<T>::ld(p); }
+    __device__ __forceinline__ void store(T* p) const { Elem<T>::st(p, v); }
+    __device__ __forceinline__ float get(int) const { return v; }
+  };
+};
+template <typename T> using GnX = typename GnTypes<T>::X;
+template <typename T> using GnE = typename GnTypes<T>::E;
+
 // all elements of a vector at once: two bf16 in one conversion
 __device__ __forceinline__ void gn_pack(Vec16<float>& x, const float (&v)[4]) { x.raw = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void gn_pack(Vec16<bf16_t>& x, const float (&v)[8]) {
@@ -227,6 +250,8 @@ __device__ __forceinline__ void gn_pack_exact(Vec16<bf16_t>& x, const float (&v)
 #pragma unroll
   for (int e = 0; e < 8; e += 2) ((uint32_t*)&x.raw)[e >> 1] = __builtin_amdgcn_perm(__float_as_uint(v[e + 1]), __float_as_uint(v[e]), 0x07060302u);
 }
+template <typename X> __device__ __forceinline__ void gn_pack(X& x, const float (&v)[1]) { x.v = v[0]; }
+template <typename X> __device__ __forceinline__ void gn_pack_exact(X& x, const float (&v)[1]) { x.v = v[0]; }
 // activations of a vector: the launch's activation is uniform, so the branch stands outside the elements
 template <int V> __device__ __forceinline__ void gn_acts(int act, float (&u)[V]) {
   if (act == ACT_RELU) {
@@ -244,7 +269,7 @@ template <int V> __device__ __forceinline__ void gn_acts(int act, float (&u)[V])
 // the block's image, chunk and range of pixels, and the thread's place in them
 template <typename T, int NT>
 struct GnPlace {
-  static constexpr int V = Vec16<T>::N;
+  static constexpr int V = GnX<T>::N;
   int n, c0, s, row, w, p0, p1;
   bool on;
   __device__ __forceinline__ GnPlace(const GnParams& p, int job) {
@@ -260,11 +285,11 @@ struct GnPlace {
   // a tensor's vector of the thread's k-th pixel: a uniform address and one 32-bit offset a lane for all k
   struct Ref {
     char* base; unsigned off; long long step;
-    __device__ __forceinline__ T* at(int k) const { return (T*)(base + k * step + off); }
+    __device__ __forceinline__ GnE<T>* at(int k) const { return (GnE<T>*)(base + k * step + off); }
   };
   __device__ __forceinline__ Ref ref(const GnParams& p, const void* t, long long cs) const {
-    return Ref{(char*)t + (((long long)n * p.HW + p0) * cs + c0) * (long long)sizeof(T), (unsigned)((row * (int)cs + w * V) * (int)sizeof(T)),
-               (long long)p.rows * cs * (long long)sizeof(T)};
+    return Ref{(char*)t + (((long long)n * p.HW + p0) * cs + c0) * (long long)sizeof(GnE<T>), (unsigned)((row * (int)cs + w * V) * (int)sizeof(GnE<T>)),
+               (long long)p.rows * cs * (long long)sizeof(GnE<T>)};
   }
   __device__ __forceinline__ int pixel(const GnParams& p, int k) const { return p0 + row + k * p.rows; }
   __device__ __forceinline__ bool has(const GnParams& p, int k) const { return on && pixel(p, k) < p1; }
@@ -383,14 +408,14 @@ constexpr int GN_AHEAD = 4;          // vectors read together where stores stand
 
 // WAY GN_ONE: the whole forward pass.  GN_TWO: moments of a range of pixels.
 template <typename T, int NT, int R, bool WHOLE, int WAY>
-__global__ void __launch_bounds__(NT, R <= 13 ? 4 : 2) gn_fwd_kernel(GnParams p) {
-  constexpr int V = Vec16<T>::N;
+__global__ void __launch_bounds__(NT, 4) gn_fwd_kernel(GnParams p) {
+  constexpr int V = GnX<T>::N;
   extern __shared__ float lds[];          // mean, rstd [groups]; partial sums
   const GnPlace<T, NT> me(p, xcd_remap(blockIdx.x, gridDim.x));
   const int g0 = me.c0 / p.cg, groups = p.W * V / p.cg, c = me.c();
   float *mean = lds, *rstd = lds + groups, *part = lds + 2 * groups;
   const auto px = me.ref(p, p.x, p.x_cs), pr = me.ref(p, p.res, p.res_cs), py = me.ref(p, p.y, p.y_cs);
-  Vec16<T> x[R];
+  GnX<T> x[R];
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (me.has(p, k)) x[k].load(px.at(k));
@@ -432,7 +457,7 @@ __global__ void __launch_bounds__(NT, R <= 13 ? 4 : 2) gn_fwd_kernel(GnParams p)
   for (int e = 0; e < V; ++e) { rg[e] = rs[e] * p.gamma[c + e]; b[e] = p.beta[c + e]; }
 #pragma unroll
   for (int k0 = 0; k0 < R; k0 += GN_AHEAD) {
-    Vec16<T> r[GN_AHEAD];
+    GnX<T> r[GN_AHEAD];
     if (p.res) {
 #pragma unroll
       for (int k = k0; k < k0 + GN_AHEAD && k < R; ++k)
@@ -457,12 +482,12 @@ __global__ void __launch_bounds__(NT, R <= 13 ? 4 : 2) gn_fwd_kernel(GnParams p)
 
 template <typename T, int NT, int R>
 __global__ void __launch_bounds__(NT) gn_fwd_apply_kernel(GnParams p) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = GnX<T>::N;
   __shared__ float mean[GN_GROUPS], rstd[GN_GROUPS];
   const GnPlace<T, NT> me(p, gridDim.x - 1 - xcd_remap(blockIdx.x, gridDim.x));
   const int g0 = me.c0 / p.cg, groups = p.W * V / p.cg;
   const auto px = me.ref(p, p.x, p.x_cs), pr = me.ref(p, p.res, p.res_cs), py = me.ref(p, p.y, p.y_cs);
-  Vec16<T> x[R], r[R];
+  GnX<T> x[R], r[R];
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (me.has(p, k)) {
@@ -499,8 +524,8 @@ __global__ void __launch_bounds__(NT) gn_fwd_apply_kernel(GnParams p) {
 // (BY_Y) or the residual.  A ReLU's dz is dy or zero and may stay in dy's registers; a smooth activation's fills no bf16.
 enum : int { GN_BY_Y = 4 };          // beside the ids of act.h
 template <int MODE, typename T, int V, typename M>
-__device__ __forceinline__ void gn_dz_vec(const Vec16<T>& x, const Vec16<T>& side, bool has_side, M& mu, M& rs, const float (&ga)[V], const float (&be)[V],
-                                          float (&dz)[V], const GnParams& p, int n, int c, const T* xp, const T* sp) {
+__device__ __forceinline__ void gn_dz_vec(const GnX<T>& x, const GnX<T>& side, bool has_side, M& mu, M& rs, const float (&ga)[V], const float (&be)[V],
+                                          float (&dz)[V], const GnParams& p, int n, int c, const GnE<T>* xp, const GnE<T>* sp) {
   if (MODE == GN_BY_Y) {
 #pragma unroll
     for (int e = 0; e < V; ++e) dz[e] = side.get(e) > 0.f ? dz[e] : 0.f;
@@ -524,7 +549,7 @@ __device__ __forceinline__ void gn_dz_vec(const Vec16<T>& x, const Vec16<T>& sid
 #pragma unroll 1
       for (int e = 0; e < V; ++e) {          // (rare: from memory again, so that it holds no registers)
         const long long q = (long long)n * p.G + (c + e) / p.cg;
-        const double u = ((double)Elem<T>::ld(xp + e) - p.mean[q]) * p.rstd[q] * p.gamma[c + e] + p.beta[c + e] + (has_side ? Elem<T>::ld(sp + e) : 0.f);
+        const double u = ((double)Elem<GnE<T>>::ld(xp + e) - p.mean[q]) * p.rstd[q] * p.gamma[c + e] + p.beta[c + e] + (has_side ? Elem<GnE<T>>::ld(sp + e) : 0.f);
         if (u > 0.0) up |= 1u << e;
       }
     }
@@ -533,7 +558,7 @@ __device__ __forceinline__ void gn_dz_vec(const Vec16<T>& x, const Vec16<T>& sid
   }
 }
 template <typename T, int V, typename M, typename P, typename R>
-__device__ __forceinline__ void gn_dz_vec(int mode, const Vec16<T>& x, const Vec16<T>& side, bool has_side, M& mu, M& rs, const float (&ga)[V],
+__device__ __forceinline__ void gn_dz_vec(int mode, const GnX<T>& x, const GnX<T>& side, bool has_side, M& mu, M& rs, const float (&ga)[V],
                                           const float (&be)[V], float (&dz)[V], const GnParams& p, const P& me, const R& px, const R& ps, int k) {
 #define GN_DZ(MODE) gn_dz_vec<MODE, T, V>(x, side, has_side, mu, rs, ga, be, dz, p, me.n, me.c(), px.at(k), ps.at(k))
   if (mode == GN_BY_Y) GN_DZ(GN_BY_Y);
@@ -589,8 +614,8 @@ __device__ __forceinline__ void gn_group_grads(const GnParams& p, int c0, int gr
 
 // The whole backward pass of a chunk but the join of the parameter gradients over images (slab [N][2][C]).
 template <typename T, int NT, int R, bool WHOLE>
-__global__ void __launch_bounds__(NT, R <= 7 ? 4 : 2) gn_bwd_kernel(GnParams p) {
-  constexpr int V = Vec16<T>::N;
+__global__ void __launch_bounds__(NT, R * sizeof(GnX<T>) <= 112 ? 4 : 2) gn_bwd_kernel(GnParams p) {
+  constexpr int V = GnX<T>::N;
   extern __shared__ float lds[];          // c1, c2 [groups]; sums of the channels [2][cw]; partial sums
   const GnPlace<T, NT> me(p, xcd_remap(blockIdx.x, gridDim.x));
   const int g0 = me.c0 / p.cg, groups = p.W * V / p.cg, c = me.c();
@@ -599,20 +624,20 @@ __global__ void __launch_bounds__(NT, R <= 7 ? 4 : 2) gn_bwd_kernel(GnParams p) 
   const int mode = p.act == ACT_RELU && p.yv ? GN_BY_Y : p.act;
   const bool smooth = p.act >= ACT_SILU;
   const auto px = me.ref(p, p.x, p.x_cs), pd = me.ref(p, p.dy, p.dy_cs), pdx = me.ref(p, p.dx, p.dx_cs), pdr = me.ref(p, p.dres, p.dres_cs);
-  Vec16<T> x[R], dy[R];
+  GnX<T> x[R], dy[R];
 #pragma unroll
   for (int k = 0; k < R; ++k)
     if (me.has(p, k)) { x[k].load(px.at(k)); dy[k].load(pd.at(k)); }
   // what the activation needs beside x: the stored output, or the residual (zeros without one)
   const void* side = p.act == ACT_NONE ? nullptr : p.yv ? p.yv : p.res;
   const auto ps = me.ref(p, side, p.yv ? p.yv_cs : p.res_cs);
-  auto read = [&](int k0, Vec16<T> (&r)[GN_AHEAD]) __attribute__((always_inline)) {
+  auto read = [&](int k0, GnX<T> (&r)[GN_AHEAD]) __attribute__((always_inline)) {
     if (!side) return;
 #pragma unroll
     for (int k = k0; k < k0 + GN_AHEAD && k < R; ++k)
       if (me.has(p, k)) r[k - k0].load(ps.at(k));
   };
-  Vec16<T> r[GN_AHEAD];
+  GnX<T> r[GN_AHEAD];
   read(0, r);
   GnVec<V, WHOLE> mu, rs;
   auto group = [&](int e) { return (long long)me.n * p.G + g0 + (me.on ? (me.w * V + e) / p.cg : 0); };
@@ -631,7 +656,7 @@ __global__ void __launch_bounds__(NT, R <= 7 ? 4 : 2) gn_bwd_kernel(GnParams p) 
 #pragma unroll
         for (int e = 0; e < V; ++e) dz[e] = dy[k].get(e);
         if (mode != ACT_NONE) {
-          gn_dz_vec(mode, x[k], r[k - k0], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
+          gn_dz_vec<T>(mode, x[k], r[k - k0], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
           if (!smooth) gn_pack_exact(dy[k], dz);
         }
 #pragma unroll
@@ -663,7 +688,7 @@ __global__ void __launch_bounds__(NT, R <= 7 ? 4 : 2) gn_bwd_kernel(GnParams p) 
 #pragma unroll
         for (int e = 0; e < V; ++e) dz[e] = dy[k].get(e);
         if (smooth) {
-          gn_dz_vec(mode, x[k], r[k - k0], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
+          gn_dz_vec<T>(mode, x[k], r[k - k0], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
           if (p.dres) gn_pack(dy[k], dz);
         }
         if (p.dres) dy[k].store(pdr.at(k));
@@ -678,7 +703,7 @@ __global__ void __launch_bounds__(NT, R <= 7 ? 4 : 2) gn_bwd_kernel(GnParams p) 
 // Sums of a range of pixels, for each channel (slab [N][S][2][C]) and each group (coef [N][S][G][2]): R pixels a thread at a time.
 template <typename T, int NT, int R, bool WHOLE>
 __global__ void __launch_bounds__(NT, 4) gn_bwd_range_kernel(GnParams p) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = GnX<T>::N;
   extern __shared__ float lds[];          // sums of the channels [2][cw]; partial sums
   GnPlace<T, NT> me(p, xcd_remap(blockIdx.x, gridDim.x));
   const int g0 = me.c0 / p.cg, groups = p.W * V / p.cg, c = me.c(), cw = p.W * V, mode = p.act == ACT_RELU && p.yv ? GN_BY_Y : p.act;
@@ -694,7 +719,7 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_range_kernel(GnParams p) {
   }
   for (; me.p0 < me.p1; me.p0 += p.rows * R) {
     const auto px = me.ref(p, p.x, p.x_cs), pd = me.ref(p, p.dy, p.dy_cs), ps = me.ref(p, side, p.yv ? p.yv_cs : p.res_cs);
-    Vec16<T> x[R], dy[R], r[R];
+    GnX<T> x[R], dy[R], r[R];
 #pragma unroll
     for (int k = 0; k < R; ++k)
       if (me.has(p, k)) {
@@ -707,7 +732,7 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_range_kernel(GnParams p) {
         float dz[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) dz[e] = dy[k].get(e);
-        if (mode != ACT_NONE) gn_dz_vec(mode, x[k], r[k], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
+        if (mode != ACT_NONE) gn_dz_vec<T>(mode, x[k], r[k], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
 #pragma unroll
         for (int e = 0; e < V; ++e) { a[e] += dz[e]; b[e] += dz[e] * (x[k].get(e) - mu[e]); }
       }
@@ -725,7 +750,7 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_range_kernel(GnParams p) {
 
 template <typename T, int NT, int R, bool WHOLE>
 __global__ void __launch_bounds__(NT, 4) gn_bwd_apply_kernel(GnParams p) {
-  constexpr int V = Vec16<T>::N;
+  constexpr int V = GnX<T>::N;
   __shared__ float c1[GN_GROUPS], c2[GN_GROUPS];
   GnPlace<T, NT> me(p, gridDim.x - 1 - xcd_remap(blockIdx.x, gridDim.x));
   const int g0 = me.c0 / p.cg, groups = p.W * V / p.cg, c = me.c();
@@ -756,7 +781,7 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_apply_kernel(GnParams p) {
   for (; me.p0 < me.p1; me.p0 += p.rows * R) {
     const auto px = me.ref(p, p.x, p.x_cs), pd = me.ref(p, p.dy, p.dy_cs), pdx = me.ref(p, p.dx, p.dx_cs), pdr = me.ref(p, p.dres, p.dres_cs);
     const auto ps = me.ref(p, side, p.yv ? p.yv_cs : p.res_cs);
-    Vec16<T> x[R], dy[R], r[R];
+    GnX<T> x[R], dy[R], r[R];
 #pragma unroll
     for (int k = 0; k < R; ++k)
       if (me.has(p, k)) {
@@ -769,7 +794,7 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_apply_kernel(GnParams p) {
         float dz[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) dz[e] = dy[k].get(e);
-        if (mode != ACT_NONE) gn_dz_vec(mode, x[k], r[k], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
+        if (mode != ACT_NONE) gn_dz_vec<T>(mode, x[k], r[k], side != nullptr, mu, rs, ga, be, dz, p, me, px, ps, k);
         if (p.dres) { gn_pack(dy[k], dz); dy[k].store(pdr.at(k)); }
 #pragma unroll
         for (int e = 0; e < V; ++e) dz[e] = rs[e] * ga[e] * dz[e] - (k1[e] + (x[k].get(e) - mu[e]) * k2[e]);
@@ -789,7 +814,8 @@ static int gn_any(const GnParams& p, bool bwd, hipStream_t s) {
     gn_apply_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
   } else {
     gn_bwd_sums_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
-    gn_bwd_coef_kernel<<<waves, 64, 0, s>>>(p);
+    const int strips = p.dgamma || p.dbeta ? (p.C + 15) / 16 : 0;
+    gn_bwd_params_kernel<<<strips + (waves + 15) / 16, 1024, 0, s>>>(p, strips);
     gn_bwd_dx_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
   }
   return 0;
@@ -799,45 +825,67 @@ static int gn_any(const GnParams& p, bool bwd, hipStream_t s) {
 // (W <= 256, rows * W <= NT).
 template <typename T, int NT, int R, bool WHOLE, int WAY>
 static void gn_fwd(const GnParams& p, int grid, int rows, hipStream_t s) {
-  gn_fwd_kernel<T, NT, R, WHOLE, WAY><<<grid, NT, 4 * (2 * (p.W * Vec16<T>::N / p.cg) + rows * p.W * (WHOLE ? 1 : Vec16<T>::N)), s>>>(p);
+  gn_fwd_kernel<T, NT, R, WHOLE, WAY><<<grid, NT, 4 * (2 * (p.W * GnX<T>::N / p.cg) + rows * p.W * (WHOLE ? 1 : GnX<T>::N)), s>>>(p);
 }
 template <typename T, int NT, int R, bool WHOLE>
 static void gn_bwd(const GnParams& p, int grid, int rows, hipStream_t s) {
-  gn_bwd_kernel<T, NT, R, WHOLE><<<grid, NT, 4 * (2 * (p.W * Vec16<T>::N / p.cg) + 2 * p.W * Vec16<T>::N * (1 + rows)), s>>>(p);
+  gn_bwd_kernel<T, NT, R, WHOLE><<<grid, NT, 4 * (2 * (p.W * GnX<T>::N / p.cg) + 2 * p.W * GnX<T>::N * (1 + rows)), s>>>(p);
 }
 
 template <typename T, int NT, int R, bool WHOLE>
 static void gn_bwd_two(const GnParams& p, int grid, int rows, hipStream_t s) {
-  gn_bwd_range_kernel<T, NT, R, WHOLE><<<grid, NT, 4 * 2 * p.W * Vec16<T>::N * (1 + rows), s>>>(p);
+  gn_bwd_range_kernel<T, NT, R, WHOLE><<<grid, NT, 4 * 2 * p.W * GnX<T>::N * (1 + rows), s>>>(p);
   gn_bwd_apply_kernel<T, NT, R, WHOLE><<<grid, NT, 0, s>>>(p);
 }
 
 template <typename T>
+static int gn_sizes(const GnParams& p, bool bwd, hipStream_t s) {
+  constexpr int V = GnX<T>::N;
+  const bool whole = p.cg % V == 0;
+  const int grid = p.N * p.S * (p.C / (p.W * V)), rows = gn_even(p.W) ? p.threads / 64 : p.rows;          // rows of partial sums
+  const int which = p.way * 1000000 + bwd * 500000 + p.threads * 100 + p.R;
+#define GN_FWD(WAY, NT, R) case WAY * 1000000 + NT * 100 + R: if (whole) gn_fwd<T, NT, R, true, WAY>(p, grid, rows, s); else gn_fwd<T, NT, R, V == 1, WAY>(p, grid, rows, s); break;
+#define GN_BWD(WAY, NT, R) case WAY * 1000000 + 500000 + NT * 100 + R: if (whole) gn_bwd<T, NT, R, true>(p, grid, rows, s); else gn_bwd<T, NT, R, V == 1>(p, grid, rows, s); break;
+#define GN_BOTH(WAY, NT, R) GN_FWD(WAY, NT, R) GN_BWD(WAY, NT, R)
+  if constexpr (V > 1) {
+    switch (which) {
+      GN_BOTH(GN_ONE, 256, 1) GN_BOTH(GN_ONE, 256, 2) GN_BOTH(GN_ONE, 512, 4) GN_BOTH(GN_ONE, 512, 7) GN_BOTH(GN_ONE, 512, 13) GN_FWD(GN_ONE, 1024, 13)
+      case GN_TWO * 1000000 + 512 * 100 + 8:
+        if (whole) gn_fwd<T, 512, 8, true, GN_TWO>(p, grid, rows, s); else gn_fwd<T, 512, 8, false, GN_TWO>(p, grid, rows, s);
+        gn_fwd_apply_kernel<T, 512, 8><<<grid, 512, 0, s>>>(p);
+        break;
+      case GN_TWO * 1000000 + 500000 + 512 * 100 + 2:
+        if (whole) gn_bwd_two<T, 512, 2, true>(p, grid, rows, s); else gn_bwd_two<T, 512, 2, false>(p, grid, rows, s);
+        break;
+      default: return (int)hipErrorInvalidValue;
+    }
+  } else {
+    switch (which) {
+      GN_BOTH(GN_LONE, 256, 4) GN_BOTH(GN_LONE, 512, 16)
+      default: return (int)hipErrorInvalidValue;
+    }
+  }
+#undef GN_BOTH
+#undef GN_FWD
+#undef GN_BWD
+  return 0;
+}
+
+template <typename T>
 static int gn_launch(const GnParams& p, bool bwd, hipStream_t s) {
+  int rc = 0;
   if (p.way == GN_ANY) {
     const bool res = p.res || p.dres;
 #define GN_CASE(A) case A: if (res) gn_any<T, A, true>(p, bwd, s); else gn_any<T, A, false>(p, bwd, s); break;
     switch (p.act) { GN_CASE(ACT_NONE) GN_CASE(ACT_RELU) GN_CASE(ACT_SILU) GN_CASE(ACT_GELU) default: return (int)hipErrorInvalidValue; }
 #undef GN_CASE
+  } else if (p.way == GN_LONE) {
+    rc = gn_sizes<Lone<T>>(p, bwd, s);
   } else {
-    constexpr int V = Vec16<T>::N;
-    const bool whole = p.cg % V == 0;
-    const int grid = p.N * p.S * (p.C / (p.W * V)), rows = gn_even(p.W) ? p.threads / 64 : p.rows;          // rows of partial sums
-    switch (p.way * 1000000 + bwd * 100000 + p.threads * 20 + p.R) {
-#define GN_FWD(NT, R, WAY) case WAY * 1000000 + NT * 20 + R: if (whole) gn_fwd<T, NT, R, true, WAY>(p, grid, rows, s); else gn_fwd<T, NT, R, false, WAY>(p, grid, rows, s); break;
-#define GN_BWD(NT, R) case GN_ONE * 1000000 + 100000 + NT * 20 + R: if (whole) gn_bwd<T, NT, R, true>(p, grid, rows, s); else gn_bwd<T, NT, R, false>(p, grid, rows, s); break;
-      GN_FWD(256, 1, GN_ONE) GN_FWD(256, 2, GN_ONE) GN_FWD(512, 4, GN_ONE) GN_FWD(512, 7, GN_ONE) GN_FWD(512, 13, GN_ONE) GN_FWD(1024, 13, GN_ONE) GN_FWD(512, 8, GN_TWO)
-      GN_BWD(256, 1) GN_BWD(256, 2) GN_BWD(512, 4) GN_BWD(512, 7) GN_BWD(512, 13)
-#undef GN_FWD
-#undef GN_BWD
-      case GN_TWO * 1000000 + 100000 + 512 * 20 + 2:
-        if (whole) gn_bwd_two<T, 512, 2, true>(p, grid, rows, s); else gn_bwd_two<T, 512, 2, false>(p, grid, rows, s);
-        break;
-      default: return (int)hipErrorInvalidValue;
-    }
-    if (!bwd && p.way == GN_TWO) gn_fwd_apply_kernel<T, 512, 8><<<grid, 512, 0, s>>>(p);
+    rc = gn_sizes<T>(p, bwd, s);
   }
-  if (bwd && (p.dgamma || p.dbeta)) gn_bwd_params_kernel<<<(p.C + 15) / 16, 1024, 0, s>>>(p);
+  if (rc) return rc;
+  if (bwd && p.way != GN_ANY && (p.dgamma || p.dbeta)) gn_bwd_params_kernel<<<(p.C + 15) / 16, 1024, 0, s>>>(p, (p.C + 15) / 16);
   return dpa_launch_rc();
 }
 

@@ -63,12 +63,13 @@ def _cdiv(a, b):
 
 
 # ----------------------------------------------------------------------------------------- group norm
-_ANY, _ONE, _TWO = 0, 1, 2          # csrc/hip/group_norm.hip
+_ANY, _ONE, _TWO, _LONE = 0, 1, 2, 3          # csrc/hip/group_norm.hip
 _plans = {}
 
 
 def _gn_plan(n, hw, c, cg, v, bwd):
-    """(way, threads, W, rows, R, S, pixels of a split) of csrc/hip/group_norm.hip for vectors of v channels (0: any layout).
+    """(way, threads, W, rows, R, S, pixels of a split) of csrc/hip/group_norm.hip for vectors of v channels (1: layouts without
+    16-byte vectors; 0: any layout).
 
     A block that holds its chunk of an image in registers reads everything once, so it is taken wherever an image fits: the
     chunk as wide as possible, down to 32 bytes of a pixel (times in us, relu + residual, 64 images, bf16; the other side is
@@ -76,8 +77,11 @@ def _gn_plan(n, hw, c, cg, v, bwd):
     124.4; 56 x 56 x 256 forward in 64 bytes 79.7, two passes 88.3, backward in 32 bytes 184, two passes 229.
     Few images make too few blocks: then the chunk is as narrow as it goes (4 images of 28 x 28 x 512: 7.1 forward and 15.1
     backward, 10.5 and 21.3 in 128 bytes), and a large image goes through two passes (4 of 56 x 56 x 256: 15.5 and 25.9, one
-    pass 19.9 and 30.4; with 16 images 26.3 and 69.2, one pass 21.7 and 49.5)."""
-    if v:
+    pass 19.9 and 30.4; with 16 images 26.3 and 69.2, one pass 21.7 and 49.5).
+    Without 16-byte vectors a lane holds one channel; up to 16 pixels a lane that is faster than the kernels for any layout
+    (64 images of 22 x 22 x 90, fp32: 12.6 forward and 16.1 backward, 17.2 and 24.4), with 52 it is not (31 x 31 x 90, bf16 with
+    a residual: 33.1 and 63.4, 24.7 and 44.7)."""
+    if v > 1:
         unit = cg * v // math.gcd(cg, v) // v          # vectors of the smallest chunk of whole groups
         total = c // v
         chunks = [w for w in range(unit, min(total, 256) + 1, unit) if total % w == 0]
@@ -95,6 +99,12 @@ def _gn_plan(n, hw, c, cg, v, bwd):
             rows, r = 512 // w, 2 if bwd else 8
             pps = rows * r * (max(1, n * _cdiv(hw, rows * r) * (total // w) // 1024) if bwd else 1)
             return _TWO, 512, w, rows, r, _cdiv(hw, pps), pps
+    if v:
+        for want in (32, 16, 1) if n * c >= 8192 else (1,):
+            for threads, r in ((256, 4), (512, 16)):
+                for w in range(cg, min(c, threads) + 1, cg):
+                    if c % w == 0 and (w >= want or w == c) and hw <= threads // w * r:
+                        return _LONE, threads, w, threads // w, r, 1, hw
     blocks = n * _cdiv(c, 64)
     s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64))
     pps = _cdiv(hw, s)
@@ -108,8 +118,12 @@ def _gn(x, groups, vecs, spans, bwd, a, eps=0.0):
     f32 = x.dtype is _F32
     v, bits = (4 if f32 else 8), 0
     for s in spans:
-        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 20)          # (offsets of a lane in 32 bits)
-    key = (n, h * w, c, groups, 0 if bits & 15 or c % v else v, bwd)
+        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 20) << 62          # (offsets of a lane in 32 bits)
+    if bits >> 62:
+        v = 0
+    elif bits & 15 or c % v:
+        v = 1
+    key = (n, h * w, c, groups, v, bwd)
     plan = _plans.get(key)
     if plan is None:
         if len(_plans) > 4096:
@@ -136,7 +150,7 @@ def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", resid
     p.x, p.x_cs, _ = xs
     p.y, p.y_cs, _ = ys
     p.res, p.res_cs, _ = rs
-    slab = 0 if p.way == _ONE else p.N * p.S * 2 * (p.G if p.way == _TWO else p.C)
+    slab = 0 if p.way & 1 else p.N * p.S * 2 * (p.G if p.way == _TWO else p.C)
     _run(x.device, _gn_launch, p, x, slab, 0, 0)
     return y
 
@@ -159,7 +173,7 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
     p.res, p.res_cs, _ = rs
     p.dres, p.dres_cs, _ = drs
     slab = p.N * p.S * 2 * p.C if p.way == _ANY or dgamma is not None or dbeta is not None else 0
-    coef = 0 if p.way == _ONE else 2 * p.N * p.G * (p.S if p.way == _TWO else 1)
+    coef = 0 if p.way & 1 else 2 * p.N * p.G * (p.S if p.way == _TWO else 1)
     _run(x.device, _gn_launch, p, x, slab, coef, 1)
     return dx
 
