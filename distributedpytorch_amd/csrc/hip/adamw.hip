@@ -13,7 +13,7 @@
 // the caches, pass them by (nontemporal), and many short-lived blocks keep more requests in flight than 2048 long ones: 25.6
 // million parameters with p16 159 us in 2048 blocks with cached accesses, 147 in 16384, 133 (5.8 TB/s) with nontemporal ones.
 // The 8-bit kernel computes some 110 instructions an element beside its bytes: 132.9 million parameters 528 us with
-// IEEE square roots, divisions and rounding by ldexp in 2048 blocks, 499 in 16384, 460 (5.3 TB/s) with the forms below; one
+// IEEE square roots, divisions and rounding by ldexp in 2048 blocks, 499 in 16384, 467 (5.2 TB/s) with the forms below; one
 // block a vector, or 4 elements a lane, was no faster (458, 487).
 #include "common.h"
 #include <algorithm>
@@ -39,9 +39,14 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const float* __restrict__ 
 // FAST: square root and reciprocal of the hardware, one unit in the last place each, of an update that is added to a parameter
 template <bool FAST>
 __device__ __forceinline__ float adamw_one(const AdamwScalars& a, float lr, float keep, float p, float g, float& m, float& v) {
-  g *= a.gs;
-  m += a.omb1 * (g - m);
-  v = a.b2 * v + a.omb2 * g * g;
+  {
+    // (rounded operation by operation: an 8-bit code follows from the last bits of a moment, and so it is the same wherever this
+    // formula is computed in fp32)
+#pragma clang fp contract(off)
+    g = g * a.gs;
+    m = m + a.omb1 * (g - m);
+    v = a.b2 * v + a.omb2 * g * g;
+  }
   if (FAST) {
     const bool small = v < 0x1p-96f;          // (the hardware's root of a denormal number is 0)
     const float root = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.f);
@@ -88,16 +93,15 @@ __device__ __forceinline__ uint32_t adamw_mix(uint32_t h) {        // finalizer 
   return h ^ (h >> 16);
 }
 
-// |t| * inv rounded to a multiple of its binade's step, up with the probability of the remainder: the 16 random bits and a
-// half are added to the mantissa bits below the step, which are cut off.  Below 2^LEAST the step stays the same: 2^LEAST is
-// added first and taken off again.  (The largest value `top` has no bits below its step, so nothing is rounded above it.)
+// |t| * inv rounded to a multiple of its binade's step, up with the probability of the remainder (u in (0, 1)).  Below 2^LEAST
+// the step stays the same.  The step and its inverse are powers of two made from the exponent bits: no product here rounds.
 template <int LEAST, int BITS>
-__device__ __forceinline__ float adamw_round(float t, float inv, float top, uint32_t r16) {
+__device__ __forceinline__ float adamw_round(float t, float inv, float top, float u) {
   float y = fabsf(t) * inv;
   y = y < top ? y : top;                                   // (also NaN)
-  const float least = __uint_as_float((uint32_t)(LEAST + 127) << 23), base = y < least ? least : 0.f;
-  const uint32_t q = __float_as_uint(y + base) + (r16 << (7 - BITS)) + (1u << (6 - BITS));
-  return __uint_as_float(q & ~((1u << (23 - BITS)) - 1)) - base;
+  const uint32_t e = max(__float_as_uint(y) & 0x7F800000u, (uint32_t)(LEAST + 127) << 23);
+  const float q = floorf(y * __uint_as_float(((uint32_t)(254 + BITS) << 23) - e) + u) * __uint_as_float(e - ((uint32_t)BITS << 23));
+  return q < top ? q : top;
 }
 
 __device__ __forceinline__ float adamw_block_max(float a) {        // over the 8 lanes that share a block
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
     }
     am = adamw_block_max(am); av = adamw_block_max(av);
     const bool some_m = am >= 0x1p-100f, some_v = av >= 0x1p-100f;
-    const float im = some_m ? 448.f / am : 0.f, iv = some_v ? 57344.f / av : 0.f;
+    const float im = some_m ? 1.f / am * 448.f : 0.f, iv = some_v ? 1.f / av * 57344.f : 0.f;
     uint32_t mo[2] = {0, 0}, vo[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
@@ -150,8 +154,8 @@ __global__ void __launch_bounds__(256) adamw8_kernel(float* __restrict__ p, cons
       for (int j = 0; j < 2; ++j) {
         const unsigned long long at = (unsigned long long)(first + i + k + j);
         const uint32_t r = adamw_mix((uint32_t)at ^ key ^ ((uint32_t)(at >> 32) * 0x85EBCA6Bu));
-        qm[j] = copysignf(adamw_round<-6, 3>(mv[k + j], im, 448.f, r & 0xFFFFu), mv[k + j]);
-        qv[j] = adamw_round<-14, 2>(vv[k + j], iv, 57344.f, r >> 16);
+        qm[j] = copysignf(adamw_round<-6, 3>(mv[k + j], im, 448.f, ((float)(r & 0xFFFFu) + 0.5f) * 0x1p-16f), mv[k + j]);
+        qv[j] = adamw_round<-14, 2>(vv[k + j], iv, 57344.f, ((float)(r >> 16) + 0.5f) * 0x1p-16f);
         if (vv[k + j] > 0.f && some_v) qv[j] = fmaxf(qv[j], 0x1p-16f);
       }
       // (both values are representable: these conversions round nothing)

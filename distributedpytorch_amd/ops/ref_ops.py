@@ -692,10 +692,8 @@ def adamw8_encode(t, u, which):
     most = torch.where(torch.isfinite(b), b.abs(), torch.zeros_like(b)).amax(1, keepdim=True)
     some = most >= 2.0 ** -100
     y = torch.nan_to_num(b.abs() * torch.where(some, top / most, torch.zeros_like(most)), nan=top, posinf=top).clamp_max(top)
-    base = torch.where(y < 2.0 ** least, 2.0 ** least, 0.0)          # (below 2^least the step stays the same)
-    low = 23 - bits                                                   # mantissa bits below a code's step
-    raw = (y + base).view(torch.int32) + (u.reshape(b.shape) * 2.0 ** low).to(torch.int32)
-    q = (raw >> low << low).view(torch.float32) - base
+    e = (torch.frexp(y).exponent - 1).clamp_min(least)                # (below 2^least the step stays the same)
+    q = torch.ldexp(torch.floor(torch.ldexp(y, bits - e) + u.reshape(b.shape)), e - bits).clamp_max(top)
     if which == "v":
         q = torch.where((b > 0) & some, q.clamp_min(2.0 ** (least - bits)), q)
     return torch.copysign(q, b).reshape(-1).to(dtype), torch.where(some, most * (1.0 / top), torch.zeros_like(most)).reshape(-1)
