@@ -195,10 +195,12 @@ class ArenaOptimizer:
                 step = max(step, 1.0)
                 self._set_moment(spec, "m", s["momentum_buffer"])
         for key, mine in (("m_scale", self.m_scale), ("v_scale", self.v_scale)):
-            if mine is not None and torch.is_tensor(groups[0].get(key)):
-                if groups[0][key].numel() != mine.numel():
-                    raise ValueError(f"optimizer state_dict holds {groups[0][key].numel()} scales, the model has {mine.numel()}")
-                mine.copy_(groups[0][key])          # (a code times its scale, rounded, may give a scale half a step away)
+            was = groups[0].get(key)
+            if mine is not None and torch.is_tensor(was) and was.numel() == mine.numel():
+                # a code times its scale, rounded, may give a scale some units in the last place away: the saved one is exact.
+                # (Another compute type may have laid the arena out in another way: then nothing is near, and nothing taken.)
+                was = was.to(mine.device)
+                mine.copy_(torch.where((was - mine).abs() <= 2.0 ** -21 * mine, was, mine))
         self.hyper[STEP] = step
         self._host_step = int(step)
 

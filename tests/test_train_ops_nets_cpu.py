@@ -58,6 +58,20 @@ def test_8_bit_states_load_into_32_and_back():
         assert bool(((a - b).abs() <= 4 * nets.E * b).all())
 
 
+def test_8_bit_states_load_into_a_network_of_another_layout():
+    """A bf16 network pads its input to 8 channels, an fp32 one to 4: arenas of different lengths, the same states."""
+    a, b = nets.model("cpu", torch.float32, "adamw8"), nets.model("cpu", torch.bfloat16, "adamw8")
+    assert a.opt.m.numel() != b.opt.m.numel()
+    a.train_step(*nets.batch(2, a.net, torch.float32, 0))
+    sd = a.opt.state_dict()
+    b.opt.load_state_dict(sd)
+    for i, s in b.opt.state_dict()["state"].items():
+        for k in ("exp_avg", "exp_avg_sq"):          # blocks of 64 lie elsewhere: one more rounding, of half a step of the largest code
+            want = sd["state"][i][k]
+            if want.shape == s[k].shape:
+                assert nets.rel(s[k], want) <= (2.0 ** -4 if k == "exp_avg" else 2.0 ** -3)
+
+
 @pytest.mark.parametrize("make", [
     lambda: ArenaOptimizer(ParamStore("cpu").finalize(), "adamw16"),
     lambda: get_model("resnet", 10, norm="layer"),
