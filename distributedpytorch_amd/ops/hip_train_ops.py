@@ -97,8 +97,10 @@ def _gn_plan(n, hw, c, cg, v, bwd):
         if fit:
             w = next((w for w in fit if w >= 16), fit[-1])
             rows, r = 512 // w, 2 if bwd else 8
-            pps = rows * r * (max(1, n * _cdiv(hw, rows * r) * (total // w) // 1024) if bwd else 1)
-            return _TWO, 512, w, rows, r, _cdiv(hw, pps), pps
+            # (64 pixels a thread at most: sums in 32 bits; and every block of the second pass joins all S ranges)
+            pps = rows * r * (max(1, min(n * _cdiv(hw, rows * r) * (total // w) // 1024, 32)) if bwd else 1)
+            if hw <= 2048 * pps:
+                return _TWO, 512, w, rows, r, _cdiv(hw, pps), pps
     if v:
         for want in (32, 16, 1) if n * c >= 8192 else (1,):
             for threads, r in ((256, 4), (512, 16)):
@@ -106,7 +108,7 @@ def _gn_plan(n, hw, c, cg, v, bwd):
                     if c % w == 0 and (w >= want or w == c) and hw <= threads // w * r:
                         return _LONE, threads, w, threads // w, r, 1, hw
     blocks = n * _cdiv(c, 64)
-    s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64))
+    s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64), min(_cdiv(hw, 2048), 65535))          # (512 pixels a thread)
     pps = _cdiv(hw, s)
     return _ANY, 256, 1, 1, 1, _cdiv(hw, pps), pps
 
@@ -118,7 +120,7 @@ def _gn(x, groups, vecs, spans, bwd, a, eps=0.0):
     f32 = x.dtype is _F32
     v, bits = (4 if f32 else 8), 0
     for s in spans:
-        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 20) << 62          # (offsets of a lane in 32 bits)
+        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 18) << 62          # (offsets of a lane in 32 bits)
     if bits >> 62:
         v = 0
     elif bits & 15 or c % v:

@@ -202,6 +202,50 @@ def test_a_bad_value_stays_in_its_row(dtype, m, n, k):
         assert torch.equal(dwx[:, cols != 3], want[2][:, cols != 3]) and not torch.isfinite(dwx[:, 3]).any()
 
 
+def check_large(n, h, w, c, groups, dtype, view=lambda t: t):
+    """Forward and backward against the formula in 64 bits, on the GPU, where the sizes are too large for the CPU."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x, dy = (view(torch.randn(n, h, w, c, device="cuda", generator=g).to(dtype)) for _ in range(2))
+    ga, be = torch.rand(c, device="cuda", generator=g) + 0.5, torch.randn(c, device="cuda", generator=g)
+    y, dx = (view(torch.empty(n, h, w, c, device="cuda", dtype=dtype)) for _ in range(2))
+    mean, rstd, dg, db = *torch.empty(2, n * groups, device="cuda"), *torch.empty(2, c, device="cuda")
+    ops.group_norm_fwd(x, ga, be, groups, 1e-5, y, mean, rstd, act="silu")
+    ops.group_norm_bwd(dy, x, ga, be, groups, mean, rstd, dx, dg, db, act="silu")
+    half = nets.E if dtype == F32 else 2.0 ** -8
+    tol = half + 1024 * nets.E          # (512 roundings of a statistic, each way)
+    sg, sb, k = torch.zeros(c, device="cuda", dtype=torch.float64), torch.zeros(c, device="cuda", dtype=torch.float64), c // groups
+    for i in range(n):
+        xd = x[i].double().reshape(-1, groups, k)
+        mu = xd.mean((0, 2))
+        rs = 1 / ((xd - mu[:, None]).square().mean((0, 2)) + 1e-5).sqrt()
+        xh = ((xd - mu[:, None]) * rs[:, None]).reshape(-1, c)
+        u = xh * ga + be
+        s = torch.sigmoid(u)
+        assert nets.rel(y[i].reshape(-1, c), u * s) <= tol
+        dz = dy[i].double().reshape(-1, c) * s * (1 + u * (1 - s))
+        t = (dz * ga).reshape(-1, groups, k)
+        h2 = xh.reshape(-1, groups, k)
+        want = rs[:, None] * (t - t.mean((0, 2))[:, None] - h2 * (t * h2).mean((0, 2))[:, None])
+        assert nets.rel(dx[i].reshape(-1, c), want.reshape(-1, c)) <= tol
+        sg += (dz * xh).sum(0)
+        sb += dz.sum(0)
+    # a sum of n random terms is near their root: 1024 roundings of sum |dz| are sqrt(n) times as many of the sum
+    for got, want in ((dg, sg), (db, sb)):
+        assert float((got.double() - want).abs().max()) <= 1024 * nets.E * n * h * w * 3
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_group_norm_of_a_large_image(dtype):
+    check_large(1, 3000, 2100, 8, 2, dtype)
+    check_large(2, 1024, 999, 6, 3, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("wide", [(1 << 18) - 8, 1 << 18, (1 << 20) + 8])
+def test_group_norm_of_pixels_far_apart(dtype, wide):
+    check_large(2, 9, 3, 24, 3, dtype, lambda t: torch.zeros(2, 9, 3, wide, device="cuda", dtype=dtype)[..., 16: 40].copy_(t))
+
+
 def test_group_norm_beyond_31_bits_of_elements():
     """A channel slice of a wide buffer whose last image starts behind 2^31 elements, against that image alone."""
     n, h, w, c, wide = 5, 640, 512, 16, 1704
