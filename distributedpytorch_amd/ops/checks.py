@@ -245,7 +245,10 @@ def adamw(name, p, g, p16, hyper, groups, group_ids, lo, hi, states):
         raise ValueError(f"{name}: group_ids must be uint8, one for each {ARENA_BLOCK} elements, on {dev}")
     at += [hyper.data_ptr(), groups.data_ptr(), group_ids.data_ptr()]
     at += [_arena(t, name, k, dt, count, dev) for k, t, dt, count in states]
-    spans = sorted((a, a + t.numel() * t.element_size()) for a, t in zip(at[:3] + at[6:], (p, g, p16) + tuple(s[1] for s in states)) if t is not None)
+    spans = [(at[0], at[0] + 4 * n), (at[1], at[1] + 4 * n), *((a, a + t.element_size() * count) for a, (_, t, _, count) in zip(at[6:], states))]
+    if p16 is not None:
+        spans.append((at[2], at[2] + 2 * n))
+    spans.sort()
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise ValueError(f"{name}: the arenas overlap")
     return hi, at

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from ctypes import byref
 
 import torch
@@ -18,12 +19,8 @@ from .native import F32, I32, I64, VP
 _F32, _BF16 = torch.float32, torch.bfloat16
 
 
-class GnParams(ctypes.Structure):
-    _fields_ = [("x", VP), ("res", VP), ("dy", VP), ("yv", VP), ("y", VP), ("dx", VP), ("dres", VP), ("gamma", VP), ("beta", VP),
-                ("mean", VP), ("rstd", VP), ("slab", VP), ("coef", VP), ("dgamma", VP), ("dbeta", VP),
-                ("x_cs", I64), ("res_cs", I64), ("dy_cs", I64), ("yv_cs", I64), ("y_cs", I64), ("dx_cs", I64), ("dres_cs", I64),
-                ("N", I32), ("HW", I32), ("C", I32), ("G", I32), ("cg", I32), ("S", I32), ("pps", I32),
-                ("act", I32), ("W", I32), ("rows", I32), ("R", I32), ("threads", I32), ("way", I32), ("eps", F32)]
+# GnParams of csrc/hip/group_norm.hip: 15 addresses, 7 strides, 13 integers, eps
+_GN_PARAMS = struct.Struct("@15Q7q13if")
 
 
 class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
@@ -43,8 +40,12 @@ def _lib():
     if _loaded:
         return _loaded[0]
     lib = native.hip_lib()
-    if lib.dpa_gn_params_size() != ctypes.sizeof(GnParams) or lib.dpa_lin_params_size() != ctypes.sizeof(LinCall):
+    if lib.dpa_gn_params_size() != _GN_PARAMS.size or lib.dpa_lin_params_size() != ctypes.sizeof(LinCall):
         raise RuntimeError("GnParams / LinCall ABI mismatch between ops/hip_train_ops.py and csrc/hip")
+    for name, types in (("dpa_group_norm", (ctypes.c_char_p, I32, I32, VP)), ("dpa_linear", (VP, VP)),
+                        ("dpa_adamw_step", (VP,) * 7 + (I32, VP, I64, VP)),
+                        ("dpa_adamw8_step", (VP,) * 9 + (I32, VP, ctypes.c_uint, I64, I64, VP))):
+        lib.declare(name, types)          # (plain integers are converted faster than wrapped ones)
     _loaded.append(lib)
     return lib
 
@@ -53,9 +54,9 @@ def _run(device, body, *args):
     """body(stream, *args) with the tensors' device as the current one, on its current stream"""
     i = device.index
     if i == torch._C._cuda_getDevice():
-        return body(VP(torch._C._cuda_getCurrentRawStream(i)), *args)
+        return body(torch._C._cuda_getCurrentRawStream(i), *args)
     with torch.cuda.device(device):
-        return body(VP(torch._C._cuda_getCurrentRawStream(i)), *args)
+        return body(torch._C._cuda_getCurrentRawStream(i), *args)
 
 
 def _cdiv(a, b):
@@ -113,47 +114,47 @@ def _gn_plan(n, hw, c, cg, v, bwd):
     return _ANY, 256, 1, 1, 1, _cdiv(hw, pps), pps
 
 
-def _gn(x, groups, vecs, spans, bwd, a, eps=0.0):
+def _gn(x, groups, spans, vecs, grads, bwd, a, eps):
+    """spans: of x, residual, dy, y (the mask), y (the output), dx, dresidual; grads: the addresses of dgamma and dbeta."""
     n, h, w, c = x.shape
-    p = GnParams()
-    p.gamma, p.beta, p.mean, p.rstd = vecs[:4]
     f32 = x.dtype is _F32
-    v, bits = (4 if f32 else 8), 0
-    for s in spans:
-        bits |= s[0] | s[1] * (4 if f32 else 2) | (s[1] >= 1 << 18) << 62          # (offsets of a lane in 32 bits)
-    if bits >> 62:
+    (ax, sx, _), (ar, sr, _), (ad, sd, _), (am, sm, _), (ay, sy, _), (adx, sdx, _), (adr, sdr, _) = spans
+    strides = sx | sr | sd | sm | sy | sdx | sdr
+    if strides >= 1 << 18:          # (offsets of a lane in 32 bits)
         v = 0
-    elif bits & 15 or c % v:
-        v = 1
+    else:
+        v = 4 if f32 else 8
+        if (ax | ar | ad | am | ay | adx | adr | strides * (4 if f32 else 2)) & 15 or c % v:
+            v = 1
     key = (n, h * w, c, groups, v, bwd)
     plan = _plans.get(key)
     if plan is None:
         if len(_plans) > 4096:
             _plans.clear()
-        plan = _plans[key] = _gn_plan(n, h * w, c, c // groups, key[4], bwd)
-    p.N, p.HW, p.C, p.G, p.cg, p.act, p.eps = n, h * w, c, groups, c // groups, a, eps
-    p.way, p.threads, p.W, p.rows, p.R, p.S, p.pps = plan
-    return p
+        plan = _plans[key] = _gn_plan(n, h * w, c, c // groups, v, bwd)
+    way, threads, wide, rows, r, s, pps = plan
+    if bwd:
+        slab = n * s * 2 * c if way == _ANY or grads[0] or grads[1] else 0
+        coef = 0 if way & 1 else 2 * n * groups * (s if way == _TWO else 1)
+    else:
+        slab, coef = 0 if way & 1 else n * s * 2 * (groups if way == _TWO else c), 0
+    _run(x.device, _gn_launch, x.device, slab, coef, bwd, f32, (ax, ar, ad, am, ay, adx, adr) + vecs,
+         grads + (sx, sr, sd, sm, sy, sdx, sdr, n, h * w, c, groups, c // groups, s, pps, a, wide, rows, r, threads, way, eps))
 
 
-def _gn_launch(stream, p, x, slab, coef, bwd):
-    ws = torch.empty(slab + coef, device=x.device, dtype=_F32) if slab + coef else None
-    if ws is not None:
-        p.slab = ws.data_ptr()
-        p.coef = p.slab + 4 * slab
-    _lib().dpa_group_norm(byref(p), bwd, int(x.dtype is _F32), stream)
+def _gn_launch(stream, device, slab, coef, bwd, f32, head, tail):
+    at = 0
+    if slab + coef:
+        ws = torch.empty(slab + coef, device=device, dtype=_F32)
+        at = ws.data_ptr()
+    _lib().dpa_group_norm(_GN_PARAMS.pack(*head, at, at + 4 * slab, *tail), bwd, f32, stream)
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", residual=None):
     a, xs, ys, rs, vecs = checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
-    if x.numel() == 0:
-        return y
-    p = _gn(x, groups, vecs, (xs, ys, rs), 0, a, eps)
-    p.x, p.x_cs, _ = xs
-    p.y, p.y_cs, _ = ys
-    p.res, p.res_cs, _ = rs
-    slab = 0 if p.way & 1 else p.N * p.S * 2 * (p.G if p.way == _TWO else p.C)
-    _run(x.device, _gn_launch, p, x, slab, 0, 0)
+    if x.shape[0]:
+        o = checks.NOTHING
+        _gn(x, groups, (xs, rs, o, o, ys, o, o), tuple(vecs), (0, 0), 0, a, eps)
     return y
 
 
@@ -161,22 +162,12 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
                    dresidual=None):
     a, xs, dys, dxs, ys, rs, drs, vecs = checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y,
                                                                residual, dresidual)
-    if x.numel() == 0:
+    if x.shape[0] == 0:
         for t in (dgamma, dbeta):
             if t is not None:
                 t.zero_()
         return dx
-    p = _gn(x, groups, vecs, (xs, dys, dxs, ys, rs, drs), 1, a)
-    p.dgamma, p.dbeta = vecs[4:]
-    p.x, p.x_cs, _ = xs
-    p.dy, p.dy_cs, _ = dys
-    p.dx, p.dx_cs, _ = dxs
-    p.yv, p.yv_cs, _ = ys
-    p.res, p.res_cs, _ = rs
-    p.dres, p.dres_cs, _ = drs
-    slab = p.N * p.S * 2 * p.C if p.way == _ANY or dgamma is not None or dbeta is not None else 0
-    coef = 0 if p.way & 1 else 2 * p.N * p.G * (p.S if p.way == _TWO else 1)
-    _run(x.device, _gn_launch, p, x, slab, coef, 1)
+    _gn(x, groups, (xs, rs, dys, ys, checks.NOTHING, dxs, drs), tuple(vecs[:4]), tuple(vecs[4:]), 1, a, 0.0)
     return dx
 
 
@@ -328,10 +319,13 @@ def linear_wgrad(dy, x, dw, db=None, accumulate=False):
 def adamw_step(p, g, m, v, p16, hyper, groups, group_ids, lo=0, hi=None):
     n = p.numel()
     hi, at = checks.adamw("adamw_step", p, g, p16, hyper, groups, group_ids, lo, hi, (("m", m, _F32, n), ("v", v, _F32, n)))
-    ap, ag, a16, ah, agr, aid, am, av = at
+    _run(p.device, _adamw, at, groups.shape[0], lo, hi)
+
+
+def _adamw(stream, at, rows, lo, hi):
+    p, g, p16, h, gr, ids, m, v = at
     b = 4 * lo
-    _run(p.device, lambda stream: _lib().dpa_adamw_step(VP(ap + b), VP(ag + b), VP(am + b), VP(av + b), VP(a16 and a16 + 2 * lo), VP(ah), VP(agr),
-                                                        groups.shape[0], VP(aid + lo // 64), I64(hi - lo), stream))
+    _lib().dpa_adamw_step(p + b, g + b, m + b, v + b, p16 and p16 + 2 * lo, h, gr, rows, ids + lo // 64, hi - lo, stream)
 
 
 def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, seed, lo=0, hi=None):
@@ -339,8 +333,11 @@ def adamw8_step(p, g, m, v, m_scale, v_scale, p16, hyper, groups, group_ids, see
     hi, at = checks.adamw("adamw8_step", p, g, p16, hyper, groups, group_ids, lo, hi,
                           (("m", m, torch.float8_e4m3fn, n), ("v", v, torch.float8_e5m2, n), ("m_scale", m_scale, _F32, n // 64),
                            ("v_scale", v_scale, _F32, n // 64)))
-    ap, ag, a16, ah, agr, aid, am, av, ams, avs = at
+    _run(p.device, _adamw8, at, groups.shape[0], seed & 0xFFFFFFFF, lo, hi)
+
+
+def _adamw8(stream, at, rows, seed, lo, hi):
+    p, g, p16, h, gr, ids, m, v, ms, vs = at
     b, s = 4 * lo, lo // 16
-    _run(p.device, lambda stream: _lib().dpa_adamw8_step(VP(ap + b), VP(ag + b), VP(am + lo), VP(av + lo), VP(ams + s), VP(avs + s),
-                                                         VP(a16 and a16 + 2 * lo), VP(ah), VP(agr), groups.shape[0], VP(aid + lo // 64),
-                                                         ctypes.c_uint(seed & 0xFFFFFFFF), I64(lo), I64(hi - lo), stream))
+    _lib().dpa_adamw8_step(p + b, g + b, m + lo, v + lo, ms + s, vs + s, p16 and p16 + 2 * lo, h, gr, rows, ids + lo // 64, seed, lo,
+                           hi - lo, stream)

@@ -83,6 +83,10 @@ class _CheckedLib:
         self._lib = lib
         self._cache = {}
 
+    def declare(self, name, types):
+        """The types of an entry point's arguments, so that plain integers may be passed."""
+        getattr(self._lib, name).argtypes = types
+
     def __getattr__(self, name):
         fn = self._cache.get(name)
         if fn is None:
