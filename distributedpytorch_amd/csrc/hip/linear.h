@@ -21,7 +21,8 @@ struct LinParams {
   const void *addend, *pre;             // pre: z of the activation whose derivative is multiplied in
   void *out, *preact;
   float* ws;                            // [splits][rows][cols] partial products where splits > 1
-  float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns: the bias gradient), or null
+  float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns), or null
+  float* db;                            // [rows] what they are joined into: the bias gradient
   long long ld_add, ld_pre, ld_out, ld_z;
   int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
 };
@@ -173,8 +174,8 @@ __device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int
 // all but this wave's newest N pieces have landed and its LDS reads are done; behind the barrier, everyone's
 template <int N> __device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// a kernel that can make the row sums on its way (the 256 x 256 tile has no registers for them, fp32 has three parts)
-template <int MT, int P, int EPI> constexpr bool lin_sums() { return EPI == EPI_WGRAD && P == 1 && MT <= 4; }
+// a kernel that can make the row sums on its way (the 256 x 256 tile has no registers for them)
+template <int MT, int EPI> constexpr bool lin_sums() { return EPI == EPI_WGRAD && MT <= 4; }
 
 // The blocks are persistent and see ONE stream of K steps across their tiles, S of them in LDS: while step s is multiplied, the
 // steps behind it land, and step s + S is requested as soon as the buffer of step s is free, also when it belongs to the next
@@ -278,6 +279,28 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    // Sums of a's rows on the matrix pipe: a times ones, an accumulator for each row tile (one for all, with ones in a column
+    // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
+    // 2 MT of them in a step of `takers`.  8192 x 4096 x 1024 with the bias gradient: 99 us, with a pass of its own over dy
+    // 110, without 95.
+    constexpr bool SUMS = lin_sums<MT, EPI>();
+    f32x4 sums[SUMS ? MT : 1];
+#pragma unroll
+    for (int i = 0; i < (SUMS ? MT : 1); ++i) sums[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int taker = j0 / BN * WN + wn;
+    const bool takes = SUMS && p.sums && taker < p.takers;
+    int turn = takes ? taker : 0x7fffffff;
+    auto add_rows = [&](auto fragment, int count) __attribute__((always_inline)) {
+      if constexpr (SUMS) {
+        if (--turn < 0) {          // (one branch a step: the steps without it lose nothing)
+          turn = p.takers - 1;
+#pragma unroll
+          for (int q = 0; q < count; ++q)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sums[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fragment(q, i), (bf16x8)(short)0x3F80, sums[i], 0, 0, 0);
+        }
+      }
+    };
     if constexpr (P == 1) {
       bf16x8 fa[MT], fb[2][NT];
       auto read_a = [&](int half, int ks) __attribute__((always_inline)) {
@@ -294,17 +317,6 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
           for (int j = 0; j < NT; ++j) mfma(fb[ks][j], fa[half * H + i], acc[half * H + i][j]);
       };
-      // Sums of a's rows on the matrix pipe: a times ones, an accumulator for each row tile (one for all, with ones in a column
-      // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
-      // 2 MT of them in a step of `takers`.  8192 x 4096 x 1024 with the bias gradient: 99 us, with a pass of its own over dy
-      // 110, without 95.
-      constexpr bool SUMS = lin_sums<MT, P, EPI>();
-      f32x4 sums[SUMS ? MT : 1];
-#pragma unroll
-      for (int i = 0; i < (SUMS ? MT : 1); ++i) sums[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      const int taker = j0 / BN * WN + wn;
-      const bool takes = SUMS && p.sums && taker < p.takers;
-      int turn = takes ? taker : 0x7fffffff;
       read_b(0);
       read_a(0, 0);
       for (; steps > 0; --steps) {
@@ -317,16 +329,7 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         __builtin_amdgcn_sched_barrier(0);
         read_a(1, 1);
         multiply(0, 1);
-        if constexpr (SUMS) {
-          if (--turn < 0) {          // (one branch a step, and fragments of its own: the steps without it lose nothing)
-            turn = p.takers - 1;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-              for (int i = 0; i < MT; ++i)
-                sums[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_at(buf, 0, i, ks), (bf16x8)(short)0x3F80, sums[i], 0, 0, 0);
-          }
-        }
+        add_rows([&](int ks, int i) { return a_at(buf, 0, i, ks); }, 2);          // (fragments of its own)
         lin_sync<(S - 2) * PP>();
         buf = buf + 1 == S ? 0 : buf + 1;
         if (steps > 1) {
@@ -342,17 +345,6 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         }
         requested();
         __builtin_amdgcn_sched_barrier(0);
-      }
-      if constexpr (SUMS) {
-        if (takes && (lane & 15) == 0) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int row = i0 + (wm * MT + i) * 16 + (lane >> 4) * 4 + e;
-              if (row < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + row] = sums[i][e];
-            }
-        }
       }
     } else {
       struct Parts { bf16x8 a[P][MT], b[P][NT]; } even, odd;
@@ -377,6 +369,7 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
           if (n % EACH == 0 && n / EACH < PP) { request(n / EACH); __builtin_amdgcn_sched_barrier(0); }
           mfma(f.b[(0x010120 >> (q * 4)) & 15][j], f.a[(0x001102 >> (q * 4)) & 15][i], acc[i][j]);
         }
+        add_rows([&](int q, int i) { return f.a[P - 1 - q][i]; }, P);
         requested();
         __builtin_amdgcn_sched_barrier(0);
       };
@@ -386,6 +379,18 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
         step(odd, even, steps > 2);
       }
       if (steps) step(even, odd, false);
+    }
+
+    if constexpr (SUMS) {
+      if (takes && (lane & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = i0 + (wm * MT + i) * 16 + (lane >> 4) * 4 + e;
+            if (row < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + row] = sums[i][e];
+          }
+      }
     }
 
     // ---- epilogue, from registers.  Neighbouring 16-column tiles trade quarters, so that a lane holds 8 columns of one row,
@@ -466,13 +471,32 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // no piece is on its way to LDS that is no longer this block's
 }
 
-// joins the partial products of a split reduction in a fixed order and applies the epilogue
+// joins partial sums [parts][cols] in a fixed order: 16 columns a block of 256, 16 threads over the parts of each
+__device__ __forceinline__ void lin_join_sums(const float* __restrict__ slab, int parts, int cols, int accumulate, float* __restrict__ out, int block) {
+  __shared__ float sh[16][17];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = block * 16 + tx;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int k = ty; k < parts; k += 16) s += slab[(long long)k * cols + c];
+  }
+  sh[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < cols) {
+    for (int k = 1; k < 16; ++k) s += sh[k][tx];
+    out[c] = accumulate ? out[c] + s : s;
+  }
+}
+
+// joins the partial products of a split reduction in a fixed order and applies the epilogue; the blocks behind the first `main`
+// ones join the bias gradient
 template <typename T, int EPI>
-__global__ void __launch_bounds__(256) lin_join_kernel(LinParams p) {
+__global__ void __launch_bounds__(256) lin_join_kernel(LinParams p, int main) {
+  if ((int)blockIdx.x >= main) return lin_join_sums(p.sums, p.splits * p.takers, p.rows, p.accumulate, p.db, blockIdx.x - main);
   const int groups = (p.cols + 7) / 8;
   const long long total = (long long)p.rows * groups, part = (long long)p.rows * p.cols;
   const bool whole = (p.cols & 7) == 0;
-  for (long long t = blockIdx.x * 256LL + threadIdx.x; t < total; t += gridDim.x * 256LL) {
+  for (long long t = blockIdx.x * 256LL + threadIdx.x; t < total; t += main * 256LL) {
     const int i = (int)(t / groups), j = (int)(t - (long long)i * groups) * 8, n = min(8, p.cols - j);
     float v[8] = {};
 #pragma unroll 4
@@ -510,7 +534,10 @@ static int lin_run(const LinParams& p, hipStream_t s) {
   }
   const int grid = (int)(jobs < 256 * residents ? jobs : 256 * residents);
   lin_mfma_kernel<T, WM, WN, MT, NT, S, P, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
-  if (p.splits > 1) lin_join_kernel<T, EPI><<<dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256), 256, 0, s>>>(p);
+  if (p.splits > 1) {
+    const int main = dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256);
+    lin_join_kernel<T, EPI><<<main + (p.sums ? (p.rows + 15) / 16 : 0), 256, 0, s>>>(p, main);
+  }
   return dpa_launch_rc();
 }
 

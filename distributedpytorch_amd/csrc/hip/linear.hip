@@ -88,21 +88,8 @@ __global__ void __launch_bounds__(256) lin_colsum_kernel(const T* __restrict__ x
     }
   }
 }
-// 16 columns a block, 16 threads over the rows of the slab for each
-__global__ void __launch_bounds__(256) lin_colsum_join_kernel(const float* __restrict__ slab, int splits, int cols, int accumulate, float* __restrict__ out) {
-  __shared__ float sh[16][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
-  float s = 0.f;
-  if (c < cols) {
-#pragma unroll 4
-    for (int k = ty; k < splits; k += 16) s += slab[(long long)k * cols + c];
-  }
-  sh[ty][tx] = s;
-  __syncthreads();
-  if (ty == 0 && c < cols) {
-    for (int k = 1; k < 16; ++k) s += sh[k][tx];
-    out[c] = accumulate ? out[c] + s : s;
-  }
+__global__ void __launch_bounds__(256) lin_colsum_join_kernel(const float* slab, int parts, int cols, int accumulate, float* out) {
+  lin_join_sums(slab, parts, cols, accumulate, out, blockIdx.x);
 }
 
 template <typename T>
@@ -227,7 +214,8 @@ DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
     case EPI_WGRAD: rc = lin_wgrad(c.p, c.tile, s); break;
   }
   if (rc || !c.db) return rc;
-  if (c.p.sums) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.db_splits, c.a_cols, c.p.accumulate, c.db);
-  else if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
+  if (c.p.sums) {
+    if (c.p.splits == 1) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.p.takers, c.a_cols, c.p.accumulate, c.db);
+  } else if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
   return dpa_launch_rc();
 }

@@ -25,7 +25,7 @@ _GN_PARAMS = struct.Struct("@15Q7q13if")
 
 class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
     _fields_ = [("a", VP), ("b", VP), ("lda", I64), ("ldb", I64), ("a_part", I64), ("b_part", I64), ("bias", VP), ("addend", VP), ("pre", VP),
-                ("out", VP), ("preact", VP), ("ws", VP), ("sums", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
+                ("out", VP), ("preact", VP), ("ws", VP), ("sums", VP), ("db_out", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
                 ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("vec", I32),
                 ("bias_vec", I32), ("takers", I32),
                 ("src_a", VP), ("src_b", VP), ("pack_a", VP), ("pack_b", VP), ("db", VP), ("db_slab", VP), ("src_lda", I64), ("src_ldb", I64),
@@ -236,12 +236,12 @@ def _linear(stream, c, t_a, a, t_b, b, k, device):
             c.splits = _cdiv(steps, _cdiv(steps, c.splits))          # no range is empty
             need += c.splits * c.rows * c.cols * 4 + 15 & ~15
         if c.db:          # (an fprop has none)
-            if not f32 and c.tile > 0:          # the product makes the sums: 2 waves in each of the tiles of a row
-                c.takers = min(2 * _cdiv(c.cols, 64 if c.tile == 3 else 128), 16)
-                c.db_splits = c.splits * c.takers
+            if c.tile > 0:          # the product makes the sums: 2 waves in each of the tiles of a row
+                c.takers = min(2 * _cdiv(c.cols, 64 if c.tile == 3 or c.tile == 5 else 128), 16)
+                need += c.splits * c.takers * c.rows * 4
             else:
                 c.db_splits = max(1, min(_cdiv(k, 32), 1024 // _cdiv(c.rows, 512)))
-            need += c.db_splits * c.rows * 4
+                need += c.db_splits * c.rows * 4
     if need:
         ws = torch.empty(need, device=device, dtype=torch.uint8)
         at = ws.data_ptr()
@@ -255,7 +255,7 @@ def _linear(stream, c, t_a, a, t_b, b, k, device):
             c.ws = at
             at += c.splits * c.rows * c.cols * 4 + 15 & ~15
         if c.takers:
-            c.sums = at
+            c.sums, c.db_out = at, c.db
         else:
             c.db_slab = at
     _lib().dpa_linear(byref(c), stream)
