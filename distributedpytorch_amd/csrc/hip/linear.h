@@ -280,9 +280,9 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     // Sums of a's rows on the matrix pipe: a times ones, an accumulator for each row tile (one for all, with ones in a column
-    // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in each of the tiles of a row, take the steps in turn, so each makes
-    // 2 MT of them in a step of `takers`.  8192 x 4096 x 1024 with the bias gradient: 99 us, with a pass of its own over dy
-    // 110, without 95.
+    // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in
+    // each of the tiles of a row, take the steps in turn, so each pays in one step of `takers`.  bf16, 8192 x 4096 x 1024 with
+    // the bias gradient: 100 us, with a pass of its own over dy 110, without it 96; fp32, 2198 x 16 x 72: 13.9 and 13.4.
     constexpr bool SUMS = lin_sums<MT, EPI>();
     f32x4 sums[SUMS ? MT : 1];
 #pragma unroll

@@ -14,9 +14,9 @@ from ctypes import byref
 import torch
 
 from . import checks, native
-from .native import F32, I32, I64, VP
+from .native import I32, I64, VP
 
-_F32, _BF16 = torch.float32, torch.bfloat16
+_F32 = torch.float32
 
 
 # GnParams of csrc/hip/group_norm.hip: 15 addresses, 7 strides, 13 integers, eps
