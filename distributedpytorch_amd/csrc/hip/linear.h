@@ -22,7 +22,7 @@ struct LinParams {
   void *out, *preact;
   float* ws;                            // [splits][rows][cols] partial products where splits > 1
   float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns), or null
-  float* db;                            // [rows] what they are joined into: the bias gradient
+  float* db;                            // [rows] what they are joined into, the bias gradient; null: sums is it
   long long ld_add, ld_pre, ld_out, ld_z;
   int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
 };
@@ -388,7 +388,10 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int row = i0 + (wm * MT + i) * 16 + (lane >> 4) * 4 + e;
-            if (row < p.rows) p.sums[((long long)split * p.takers + taker) * p.rows + row] = sums[i][e];
+            if (row < p.rows) {
+              float* o = p.sums + ((long long)split * p.takers + taker) * p.rows + row;
+              *o = !p.db && p.accumulate ? *o + sums[i][e] : sums[i][e];
+            }
           }
       }
     }

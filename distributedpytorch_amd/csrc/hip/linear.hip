@@ -215,7 +215,7 @@ DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
   }
   if (rc || !c.db) return rc;
   if (c.p.sums) {
-    if (c.p.splits == 1) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.p.takers, c.a_cols, c.p.accumulate, c.db);
+    if (c.p.splits == 1 && c.p.db) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.p.takers, c.a_cols, c.p.accumulate, c.db);
   } else if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
   return dpa_launch_rc();
 }

@@ -9,7 +9,6 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
-from ctypes import byref
 
 import torch
 
@@ -23,14 +22,9 @@ _F32 = torch.float32
 _GN_PARAMS = struct.Struct("@15Q7q13if")
 
 
-class LinCall(ctypes.Structure):          # LinParams and LinCall of csrc/hip/linear.h
-    _fields_ = [("a", VP), ("b", VP), ("lda", I64), ("ldb", I64), ("a_part", I64), ("b_part", I64), ("bias", VP), ("addend", VP), ("pre", VP),
-                ("out", VP), ("preact", VP), ("ws", VP), ("sums", VP), ("db_out", VP), ("ld_add", I64), ("ld_pre", I64), ("ld_out", I64), ("ld_z", I64),
-                ("rows", I32), ("cols", I32), ("K", I32), ("parts", I32), ("splits", I32), ("accumulate", I32), ("act", I32), ("vec", I32),
-                ("bias_vec", I32), ("takers", I32),
-                ("src_a", VP), ("src_b", VP), ("pack_a", VP), ("pack_b", VP), ("db", VP), ("db_slab", VP), ("src_lda", I64), ("src_ldb", I64),
-                ("a_rows", I32), ("a_cols", I32), ("b_rows", I32), ("b_cols", I32), ("ld_a", I32), ("ld_b", I32), ("vec_a", I32), ("vec_b", I32),
-                ("db_splits", I32), ("epi", I32), ("tile", I32), ("f32", I32)]
+# LinCall of csrc/hip/linear.h: operands and their strides; bias, addend, pre, out, preact, workspaces; strides; ten integers; the
+# operands as they are and what they are packed into, the bias gradient and its slab; strides; twelve integers
+_LIN_CALL = struct.Struct("@2Q4q8Q4q10i6Q2q12i")
 
 
 _loaded = []
@@ -40,9 +34,9 @@ def _lib():
     if _loaded:
         return _loaded[0]
     lib = native.hip_lib()
-    if lib.dpa_gn_params_size() != _GN_PARAMS.size or lib.dpa_lin_params_size() != ctypes.sizeof(LinCall):
-        raise RuntimeError("GnParams / LinCall ABI mismatch between ops/hip_train_ops.py and csrc/hip")
-    for name, types in (("dpa_group_norm", (ctypes.c_char_p, I32, I32, VP)), ("dpa_linear", (VP, VP)),
+    if lib.dpa_gn_params_size() != _GN_PARAMS.size or lib.dpa_lin_params_size() != _LIN_CALL.size:
+        raise RuntimeError("GnParams or LinCall of csrc/hip has another size than ops/hip_train_ops.py packs")
+    for name, types in (("dpa_group_norm", (ctypes.c_char_p, I32, I32, VP)), ("dpa_linear", (ctypes.c_char_p, VP)),
                         ("dpa_adamw_step", (VP,) * 7 + (I32, VP, I64, VP)),
                         ("dpa_adamw8_step", (VP,) * 9 + (I32, VP, ctypes.c_uint, I64, I64, VP))):
         lib.declare(name, types)          # (plain integers are converted faster than wrapped ones)
@@ -50,13 +44,13 @@ def _lib():
     return lib
 
 
-def _run(device, body, *args):
+def _run(device, body, *args, **kw):
     """body(stream, *args) with the tensors' device as the current one, on its current stream"""
     i = device.index
     if i == torch._C._cuda_getDevice():
-        return body(torch._C._cuda_getCurrentRawStream(i), *args)
+        return body(torch._C._cuda_getCurrentRawStream(i), *args, **kw)
     with torch.cuda.device(device):
-        return body(torch._C._cuda_getCurrentRawStream(i), *args)
+        return body(torch._C._cuda_getCurrentRawStream(i), *args, **kw)
 
 
 def _cdiv(a, b):
@@ -203,96 +197,84 @@ def _plan(rows, cols, k, f32):
     return 3, max(1, min(512 // t64, k // 512, 16))
 
 
-def _linear(stream, c, t_a, a, t_b, b, k, device):
-    """Fills in the operands, the plan and the workspace of a call whose epilogue is set, and launches it."""
-    c.src_a, c.src_lda, _ = a
-    c.src_b, c.src_ldb, _ = b
-    c.a_rows, c.a_cols = t_a.shape
-    c.b_rows, c.b_cols = t_b.shape
-    f32 = c.f32
+def _linear(stream, epi, t_a, a, t_b, b, rows, cols, k, vec, act=0, out=checks.NOTHING, bias=0, bias_vec=0, addend=checks.NOTHING,
+            pre=checks.NOTHING, preact=checks.NOTHING, db=0, accumulate=0):
+    """The plan, the workspace and the launch of a product: matrices as the checks return them."""
+    f32 = t_a.dtype is _F32
     es = 4 if f32 else 2
-    c.vec_a = ok_a = not (a[0] | a[1] * es) & 15
-    c.vec_b = ok_b = not (b[0] | b[1] * es) & 15
-    c.K, c.parts = k, 3 if f32 else 1
-    few = c.epi == _FPROP and c.rows <= (64 if f32 else 32) and ok_a and ok_b and not (k * es) & 15
-    # (32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
-    c.a, c.lda, c.b, c.ldb = a[0], a[1], b[0], b[1]
-    need = 0
-    if few:
-        c.tile, c.splits = -1, 1
+    (src_a, src_lda, _), (src_b, src_ldb, _) = a, b
+    (a_rows, a_cols), (b_rows, b_cols) = t_a.shape, t_b.shape
+    ok_a, ok_b = not (src_a | src_lda * es) & 15, not (src_b | src_ldb * es) & 15
+    at_a, lda, at_b, ldb = src_a, src_lda, src_b, src_ldb
+    parts = 3 if f32 else 1
+    need = ld_a = ld_b = a_part = b_part = pack_a = pack_b = ws = sums = db_out = db_slab = takers = db_splits = 0
+    if epi == _FPROP and rows <= (64 if f32 else 32) and ok_a and ok_b and not (k * es) & 15:
+        # (32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
+        tile, splits = -1, 1
     else:
-        c.tile, c.splits = _plan(c.rows, c.cols, k, f32)
+        tile, splits = _plan(rows, cols, k, f32)
         # the DMA takes bf16 rows of a multiple of 8 elements at 16-byte addresses as they are; anything else is packed
-        if f32 or not ok_a or c.a_cols & 7:
-            c.ld_a = c.lda = (c.a_cols + 7) & ~7
-            c.a_part = c.a_rows * c.lda
-            need += c.parts * c.a_part * 2 + 15 & ~15
-        if f32 or not ok_b or c.b_cols & 7:
-            c.ld_b = c.ldb = (c.b_cols + 7) & ~7
-            c.b_part = c.b_rows * c.ldb
-            need += c.parts * c.b_part * 2 + 15 & ~15
-        if c.splits > 1:
-            steps = _cdiv(k, 32 if c.tile >= 4 else 64) * (6 if f32 and c.tile < 4 else 1)
-            c.splits = _cdiv(steps, _cdiv(steps, c.splits))          # no range is empty
-            need += c.splits * c.rows * c.cols * 4 + 15 & ~15
-        if c.db:          # (an fprop has none)
-            if c.tile > 0:          # the product makes the sums: 2 waves in each of the tiles of a row
-                c.takers = min(2 * _cdiv(c.cols, 64 if c.tile == 3 or c.tile == 5 else 128), 16)
-                need += c.splits * c.takers * c.rows * 4
-            else:
-                c.db_splits = max(1, min(_cdiv(k, 32), 1024 // _cdiv(c.rows, 512)))
-                need += c.db_splits * c.rows * 4
-    if need:
-        ws = torch.empty(need, device=device, dtype=torch.uint8)
-        at = ws.data_ptr()
-        if c.ld_a:
-            c.a = c.pack_a = at
-            at += c.parts * c.a_part * 2 + 15 & ~15
-        if c.ld_b:
-            c.b = c.pack_b = at
-            at += c.parts * c.b_part * 2 + 15 & ~15
-        if c.splits > 1:
-            c.ws = at
-            at += c.splits * c.rows * c.cols * 4 + 15 & ~15
-        if c.takers:
-            c.sums, c.db_out = at, c.db
-        else:
-            c.db_slab = at
-    _lib().dpa_linear(byref(c), stream)
+        if f32 or not ok_a or a_cols & 7:
+            ld_a = lda = (a_cols + 7) & ~7
+            a_part = a_rows * lda
+            pack_a, need = 1, parts * a_part * 2 + 15 & ~15
+        if f32 or not ok_b or b_cols & 7:
+            ld_b = ldb = (b_cols + 7) & ~7
+            b_part = b_rows * ldb
+            pack_b, need = need + 1, need + (parts * b_part * 2 + 15 & ~15)
+        steps = _cdiv(k, 32 if tile >= 4 else 64) * (6 if f32 and tile < 4 else 1)
+        if splits > 1:
+            splits = _cdiv(steps, _cdiv(steps, splits))          # no range is empty
+        if splits > 1:
+            ws, need = need + 1, need + (splits * rows * cols * 4 + 15 & ~15)
+        if db:
+            if tile == 0:          # a pass over dy of its own
+                db_splits = max(1, min(_cdiv(k, 32), 1024 // _cdiv(rows, 512)))
+                db_slab, need = need + 1, need + db_splits * rows * 4
+            elif splits == 1 and steps <= 16:
+                # one wave makes the sums of a row tile, into db: at most some 100 instructions more, and no launch to join them
+                # (500 x 512 x 1000: 8.2 us, joined 10.0; 128 x 64 x 64: 9.9 us a call, 14.3)
+                takers, sums = 1, db
+            else:          # the 2 waves in each of the tiles of a row take turns
+                takers = min(2 * _cdiv(cols, 64 if tile == 3 or tile == 5 else 128), 16)
+                db_out, sums, need = db, need + 1, need + splits * takers * rows * 4
+    if need:          # (offsets plus one so far)
+        base = torch.empty(need, device=t_a.device, dtype=torch.uint8)
+        at = base.data_ptr() - 1
+        if pack_a:
+            at_a = pack_a = at + pack_a
+        if pack_b:
+            at_b = pack_b = at + pack_b
+        if ws:
+            ws += at
+        if db_out:
+            sums += at
+        if db_slab:
+            db_slab += at
+    _lib().dpa_linear(_LIN_CALL.pack(
+        at_a, at_b, lda, ldb, a_part, b_part, bias, addend[0], pre[0], out[0], preact[0], ws, sums, db_out,
+        addend[1], pre[1], out[1], preact[1], rows, cols, k, parts, splits, accumulate, act, vec, bias_vec, takers,
+        src_a, src_b, pack_a, pack_b, db, db_slab, src_lda, src_ldb,
+        a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, ok_a, ok_b, db_splits, epi, tile, f32), stream)
 
 
 def linear_fprop(x, w, y, bias=None, act="none", addend=None, preact=None):
     a, xs, ws, ys, ads, zs, b = checks.linear_fprop(x, w, y, bias, act, addend, preact)
     m, k = x.shape
-    if m == 0:
-        return y
-    c = LinCall()
-    n = w.shape[0]
-    c.epi, c.rows, c.cols, c.act, c.bias = _FPROP, m, n, a, b
-    c.out, c.ld_out, _ = ys
-    c.addend, c.ld_add, _ = ads
-    c.preact, c.ld_z, _ = zs
-    f32 = c.f32 = x.dtype is _F32
-    c.vec = not (n & 7 or (ys[0] | ads[0] | zs[0] | (ys[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
-    c.bias_vec = not (n & 7 or b & 15)
-    _run(x.device, _linear, c, x, xs, w, ws, k, x.device)
+    if m:
+        n = w.shape[0]
+        vec = not (n & 7 or (ys[0] | ads[0] | zs[0] | (ys[1] | ads[1] | zs[1]) * y.element_size()) & 15)
+        _run(x.device, _linear, _FPROP, x, xs, w, ws, m, n, k, vec, a, ys, b, not (n & 7 or b & 15), ads, checks.NOTHING, zs)
     return y
 
 
 def linear_dgrad(dy, w, dx, act="none", preact=None, addend=None):
     a, dys, ws, dxs, zs, ads = checks.linear_dgrad(dy, w, dx, act, preact, addend)
     m, n = dy.shape
-    if m == 0:
-        return dx
-    c = LinCall()
-    k = w.shape[1]
-    c.epi, c.rows, c.cols, c.act = _DGRAD, m, k, a
-    c.out, c.ld_out, _ = dxs
-    c.pre, c.ld_pre, _ = zs
-    c.addend, c.ld_add, _ = ads
-    f32 = c.f32 = dy.dtype is _F32
-    c.vec = not (k & 7 or (dxs[0] | ads[0] | zs[0] | (dxs[1] | ads[1] | zs[1]) * (4 if f32 else 2)) & 15)
-    _run(dy.device, _linear, c, dy, dys, w, ws, n, dy.device)
+    if m:
+        k = w.shape[1]
+        vec = not (k & 7 or (dxs[0] | ads[0] | zs[0] | (dxs[1] | ads[1] | zs[1]) * dx.element_size()) & 15)
+        _run(dy.device, _linear, _DGRAD, dy, dys, w, ws, m, k, n, vec, a, dxs, 0, 0, ads, zs)
     return dx
 
 
@@ -305,13 +287,9 @@ def linear_wgrad(dy, x, dw, db=None, accumulate=False):
             if db is not None:
                 db.zero_()
         return dw
-    c = LinCall()
     k = x.shape[1]
-    c.epi, c.rows, c.cols, c.accumulate, c.db = _WGRAD, n, k, int(accumulate), b
-    c.out, c.ld_out, _ = dws
-    c.f32 = dy.dtype is _F32
-    c.vec = not (k & 7 or (dws[0] | dws[1] * 4) & 15)
-    _run(dy.device, _linear, c, dy, dys, x, xs, m, dy.device)
+    vec = not (k & 7 or (dws[0] | dws[1] * 4) & 15)
+    _run(dy.device, _linear, _WGRAD, dy, dys, x, xs, n, k, m, vec, out=dws, db=b, accumulate=int(accumulate))
     return dw
 
 
