@@ -62,13 +62,14 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(GnParams p) {
   }
 }
 
-// one wave per (image, group): joins S * cg partial moments
-__global__ void __launch_bounds__(64) gn_moments_kernel(GnParams p) {
+// four waves per (image, group): join S * cg partial moments
+__global__ void __launch_bounds__(256) gn_moments_kernel(GnParams p) {
+  __shared__ float sh[4][3];
   for (long long q = blockIdx.x; q < (long long)p.N * p.G; q += gridDim.x) {
     const int n = (int)(q / p.G), g = (int)(q % p.G), total = p.S * p.cg;
     const float* o = p.slab + (long long)n * p.S * 2 * p.C + g * p.cg;
     float cnt = 0.f, mean = 0.f, m2 = 0.f;
-    for (int i = threadIdx.x; i < total; i += 64) {
+    for (int i = threadIdx.x; i < total; i += 256) {
       const int s = i / p.cg;
       const float* e = o + (long long)s * 2 * p.C + (i - s * p.cg);
       gn_join(cnt, mean, m2, (float)gn_count(p, s), e[0], e[p.C]);
@@ -78,7 +79,13 @@ __global__ void __launch_bounds__(64) gn_moments_kernel(GnParams p) {
       const float cb = __shfl_xor(cnt, k, 64), mb = __shfl_xor(mean, k, 64), qb = __shfl_xor(m2, k, 64);
       gn_join(cnt, mean, m2, cb, mb, qb);
     }
-    if (threadIdx.x == 0) { p.mean[q] = mean; p.rstd[q] = 1.f / sqrtf(m2 / cnt + p.eps); }
+    if ((threadIdx.x & 63) == 0) { float* w = sh[threadIdx.x >> 6]; w[0] = cnt; w[1] = mean; w[2] = m2; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < 4; ++k) gn_join(cnt, mean, m2, sh[k][0], sh[k][1], sh[k][2]);
+      p.mean[q] = mean; p.rstd[q] = 1.f / sqrtf(m2 / cnt + p.eps);
+    }
+    __syncthreads();
   }
 }
 
@@ -139,34 +146,43 @@ __global__ void __launch_bounds__(256) gn_bwd_sums_kernel(GnParams p) {
   }
 }
 
-// one wave per (image, group): c1, c2
-__device__ __forceinline__ void gn_bwd_coef(const GnParams& p, long long first, long long step) {
-  const int lane = threadIdx.x & 63;
+// c1, c2: four waves per (image, group), four of those a block of 1024
+__device__ __forceinline__ void gn_bwd_coef(const GnParams& p, int block, int blocks, float (*sh)[2]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, four = wave >> 2;
   const float inv = 1.f / ((float)p.HW * (float)p.cg);
-  for (long long q = first; q < (long long)p.N * p.G; q += step) {
-    const int n = (int)(q / p.G), g = (int)(q % p.G), total = p.S * p.cg;
-    const float* o = p.slab + (long long)n * p.S * 2 * p.C + g * p.cg;
+  for (long long q0 = block * 4LL; q0 < (long long)p.N * p.G; q0 += blocks * 4LL) {
+    const long long q = q0 + four;
     float sa = 0.f, sb = 0.f;
+    if (q < (long long)p.N * p.G) {
+      const int n = (int)(q / p.G), g = (int)(q % p.G), total = p.S * p.cg;
+      const float* o = p.slab + (long long)n * p.S * 2 * p.C + g * p.cg;
 #pragma unroll 2
-    for (int i = lane; i < total; i += 64) {
-      const int s = i / p.cg, k = i - s * p.cg;
-      const float* e = o + (long long)s * 2 * p.C + k;
-      const float gm = p.gamma[g * p.cg + k];
-      sa += e[0] * gm; sb += e[p.C] * gm;
+      for (int i = threadIdx.x & 255; i < total; i += 256) {
+        const int s = i / p.cg, k = i - s * p.cg;
+        const float* e = o + (long long)s * 2 * p.C + k;
+        const float gm = p.gamma[g * p.cg + k];
+        sa += e[0] * gm; sb += e[p.C] * gm;
+      }
     }
     sa = wave_sum(sa); sb = wave_sum(sb);
-    if (lane == 0) { p.coef[2 * q] = sa * inv; p.coef[2 * q + 1] = sb * inv; }
+    if (lane == 0) { sh[wave][0] = sa; sh[wave][1] = sb; }
+    __syncthreads();
+    if ((threadIdx.x & 255) == 0 && q < (long long)p.N * p.G) {
+      for (int k = 1; k < 4; ++k) { sa += sh[wave + k][0]; sb += sh[wave + k][1]; }
+      p.coef[2 * q] = sa * inv; p.coef[2 * q + 1] = sb * inv;
+    }
+    __syncthreads();
   }
 }
 
 // dgamma / dbeta in the first `strips` blocks: 16 channels x 64 row lanes over the N * S rows of the slab, in a fixed order.  The
 // blocks behind them make the coefficients of dx where it has a kernel of its own for any layout: one launch for both.
 __global__ void __launch_bounds__(1024) gn_bwd_params_kernel(GnParams p, int strips) {
+  __shared__ float sh[2][64][17];
   if ((int)blockIdx.x >= strips) {
-    gn_bwd_coef(p, (long long)(blockIdx.x - strips) * 16 + (threadIdx.x >> 6), (long long)(gridDim.x - strips) * 16);
+    gn_bwd_coef(p, blockIdx.x - strips, gridDim.x - strips, (float(*)[2])sh);
     return;
   }
-  __shared__ float sh[2][64][17];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
   const int rows = p.N * p.S;
   float sa = 0.f, sb = 0.f;
@@ -216,7 +232,7 @@ __global__ void __launch_bounds__(256) gn_bwd_dx_kernel(GnParams p) {
 // Both are bound by memory: the floor is one read of every input and one write of every output, and a copy in segments of 128
 // bytes, as the chunks have them, runs at 4.5 TB/s here.  With ReLU and residual, bf16: forward 64 x 28 x 28 x 512 37.7 us,
 // 4.1 TB/s of the floor's bytes, 64 x 14 x 14 x 1024 17.5 us, 4.4 TB/s, 64 x 56 x 56 x 256 79.7 us, 3.9 TB/s (segments of 64
-// bytes); backward 64 x 28 x 28 x 512 67.8 us, 3.8 TB/s: two blocks a CU of 16 waves at 200 registers, and the arithmetic of
+// bytes); backward 64 x 28 x 28 x 512 67.8 us, 3.8 TB/s: two blocks of 8 waves a CU at 200 registers, and the arithmetic of
 // a vector, some 25 instructions an element, is the next bound, so sign and branch decisions are made once a vector.  Sums over
 // the lanes of a wave stay in registers (DPP and lane swaps): through LDS 28 x 28 x 512 backward took 84 us.
 
@@ -807,15 +823,15 @@ __global__ void __launch_bounds__(NT, 4) gn_bwd_apply_kernel(GnParams p) {
 template <typename T, int ACT, bool RES>
 static int gn_any(const GnParams& p, bool bwd, hipStream_t s) {
   const dim3 grid((p.C + 63) / 64, p.S, min(p.N, 16384));
-  const int waves = (int)min((long long)p.N * p.G, 65536LL);
+  const int groups = (int)min((long long)p.N * p.G, 65536LL);
   if (!bwd) {
     gn_stats_kernel<T><<<grid, 256, 0, s>>>(p);
-    gn_moments_kernel<<<waves, 64, 0, s>>>(p);
+    gn_moments_kernel<<<groups, 256, 0, s>>>(p);
     gn_apply_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
   } else {
     gn_bwd_sums_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
     const int strips = p.dgamma || p.dbeta ? (p.C + 15) / 16 : 0;
-    gn_bwd_params_kernel<<<strips + (waves + 15) / 16, 1024, 0, s>>>(p, strips);
+    gn_bwd_params_kernel<<<strips + (groups + 3) / 4, 1024, 0, s>>>(p, strips);
     gn_bwd_dx_kernel<T, ACT, RES><<<grid, 256, 0, s>>>(p);
   }
   return 0;
