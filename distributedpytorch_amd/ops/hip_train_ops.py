@@ -68,11 +68,11 @@ def _gn_plan(n, hw, c, cg, v, bwd):
 
     A block that holds its chunk of an image in registers reads everything once, so it is taken wherever an image fits: the
     chunk as wide as possible, down to 32 bytes of a pixel (times in us, relu + residual, 64 images, bf16; the other side is
-    two passes): 40 x 40 x 256 forward in 128 bytes 37.0, 64 bytes 40.2, two passes 52.7, backward in 64 bytes 73.6, two passes
-    124.4; 56 x 56 x 256 forward in 64 bytes 79.7, two passes 88.3, backward in 32 bytes 184, two passes 229.
-    Few images make too few blocks: then the chunk is as narrow as it goes (4 images of 28 x 28 x 512: 7.1 forward and 15.1
-    backward, 10.5 and 21.3 in 128 bytes), and a large image goes through two passes (4 of 56 x 56 x 256: 15.5 and 25.9, one
-    pass 19.9 and 30.4; with 16 images 26.3 and 69.2, one pass 21.7 and 49.5).
+    two passes): 40 x 40 x 256 forward in 128 bytes 37, 64 bytes 40, two passes 53, backward in 64 bytes 73, two passes 108;
+    56 x 56 x 256 forward in 64 bytes 79, two passes 88, backward in 32 bytes 178, two passes 188.
+    Few images make too few blocks: then the chunk is as narrow as it goes (4 images of 28 x 28 x 512: 7.1 forward and 13.2
+    backward, 10.5 and 19.1 in 128 bytes), and a large image goes through two passes (4 of 56 x 56 x 256: 15.5 and 26.8, one
+    pass 19.9 and 28.5; with 16 images 26.3 and 75.7, one pass 20.4 and 46.8).
     Without 16-byte vectors a lane holds one channel; up to 16 pixels a lane that is faster than the kernels for any layout
     (64 images of 22 x 22 x 90, fp32: 12.6 forward and 16.1 backward, 17.2 and 24.4), with 52 it is not (31 x 31 x 90, bf16 with
     a residual: 33.1 and 63.4, 24.7 and 44.7)."""
