@@ -113,7 +113,7 @@ __device__ __forceinline__ float gn_dz(const GnParams& p, long long pix, int c, 
   xhat = (x - mean) * rstd;
   if (ACT == ACT_NONE) return dy;
   if (ACT == ACT_RELU && p.yv) return Elem<T>::ld((const T*)p.yv + pix * p.yv_cs + c) > 0.f ? dy : 0.f;
-  const float r = RES ? Elem<T>::ld((const T*)p.res + pix * p.res_cs + c) : 0.f;
+  const float r = RES && p.res ? Elem<T>::ld((const T*)p.res + pix * p.res_cs + c) : 0.f;      // (RES also where only dres is there)
   const float a = xhat * g, u = a + b + r;
   if (ACT == ACT_RELU) return dy * gn_relu_slope(u, fabsf(a) + fabsf(b) + fabsf(r), x, mean, rstd, g, b, r);
   return dy * act_slope<ACT>(u);

@@ -556,7 +556,8 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
                    dresidual=None):
     """Gradients of group_norm_fwd: dx, dgamma and dbeta (fp32 [C], or None where they are not wanted) and dresidual (or
     None).  The activation's derivative is taken at values recomputed from x (and residual); for "relu" the stored output
-    may be given as y instead, its sign is then the mask.  dx may be dy or x itself, dresidual may be dy, y or residual."""
+    may be given as y instead, its sign is then the mask.  dresidual, the gradient of what stands under the activation, may be asked
+    for without a residual.  dx may be dy or x itself, dresidual may be dy, y or residual."""
     from . import checks
     checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
     if x.numel() == 0:
