@@ -109,10 +109,11 @@ class ParamStore:
         self.wprep = WeightPrep(self)       # batched per-step filter transposes / bf16 planes (nn/wprep.py)
 
     # ---------------------------------------------------------------- registration
-    def add_conv_weight(self, name, cout, cin, kh, kw, init, trainable=True, flat_logical=False):
-        """init: callable(logical_tensor[cout, cin, kh, kw]) filling it in place (torch.nn.init style)."""
+    def add_conv_weight(self, name, cout, cin, kh, kw, init, trainable=True, flat_logical=False, cin_pad=None):
+        """init: callable(logical_tensor[cout, cin, kh, kw]) filling it in place (torch.nn.init style).  cin_pad: the channels
+        its input has in memory, where that is no network input."""
         logical = (cout, cin * kh * kw) if flat_logical else (cout, cin, kh, kw)
-        spec = ParamSpec(name, logical, (pad_to(cout), kh, kw, input_pad(cin, self.compute_dtype)), "conv", trainable,
+        spec = ParamSpec(name, logical, (pad_to(cout), kh, kw, cin_pad or input_pad(cin, self.compute_dtype)), "conv", trainable,
                          meta=(cout, cin, kh, kw))
         t = torch.empty(cout, cin, kh, kw)
         init(t)

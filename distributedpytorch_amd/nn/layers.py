@@ -733,10 +733,13 @@ class Mlp:
         if n < 1:
             raise ValueError(f"{name}: an MLP has an input and an output width, got {tuple(widths)}")
         self.layers = []
+        if min(widths) < 1:
+            raise ValueError(f"{name}: widths are at least 1, got {tuple(widths)}")
         for i, (cin, cout) in enumerate(zip(widths, widths[1:])):
             at = name if n == 1 else f"{name}.{2 * i}"
+            # (the input of a later product is the output of the one before it, which is padded as activations are)
             self.layers.append((store.add_conv_weight(f"{at}.weight", cout, cin, 1, 1, kaiming_uniform_default, trainable,
-                                                      flat_logical=True),
+                                                      flat_logical=True, cin_pad=pad_to(cin) if i else None),
                                 store.add_vec(f"{at}.bias", cout, bias_default(cin), trainable)))
 
     def _w(self, spec):
@@ -748,6 +751,9 @@ class Mlp:
         n = x.data.shape[0]
         if tuple(x.data.shape) != (n, 1, 1, x.data.shape[3]):
             raise ValueError(f"an MLP takes [N, 1, 1, C], got {tuple(x.data.shape)}")
+        first = self.layers[0][0]
+        if x.data.shape[3] != first.storage_shape[3]:
+            raise ValueError(f"{first.name} takes {first.storage_shape[3]} channels in memory, got {x.data.shape[3]}")
         needs = x.needs_grad or self.trainable or (residual is not None and residual.needs_grad)
         track = ctx.grad_enabled and needs
         h, kept = x.data.view(n, -1), []          # (input, pre-activation) of every product

@@ -2,7 +2,11 @@
 import pytest
 import torch
 
+from distributedpytorch_amd.models.factory import get_model
+from distributedpytorch_amd.nn.engine import Act, Context, ParamStore, Tape
+from distributedpytorch_amd.nn.layers import Mlp
 from tests import train_ops_forms as forms
+from tests import train_ops_nets as nets
 
 
 @pytest.mark.parametrize("case", forms.DRES, ids=str)
@@ -10,3 +14,27 @@ from tests import train_ops_forms as forms
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_dresidual_without_a_residual(case, act, dtype):
     forms.check_dresidual_alone(case, act, dtype, "cpu")
+
+
+@pytest.mark.parametrize("widths", forms.NARROW, ids=str)
+def test_narrow_hidden_layers(widths):
+    forms.check_narrow_mlp(widths, "cpu")
+
+
+@pytest.mark.parametrize("hidden", [(1,), (4,), (2, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_classifier_with_narrow_hidden_layers(hidden, dtype):
+    dm = nets.model("cpu", dtype, "adamw", head_hidden=hidden)
+    dm.train_step(*nets.batch(2, dm.net, dtype, 0))
+    assert torch.isfinite(dm.net.store.p).all()
+
+
+def test_widths_and_channels_are_refused():
+    for hidden in ((0,), (8, -1)):
+        with pytest.raises(ValueError, match="widths"):
+            get_model("resnet", 10, norm="group", head_hidden=hidden)
+    store = ParamStore("cpu")
+    m = Mlp(store, "m", (16, 8))
+    store.finalize()
+    with pytest.raises(ValueError, match="m.weight takes 16 channels"):
+        m(Context(store, True, Tape()), Act(torch.zeros(2, 1, 1, 24), False))

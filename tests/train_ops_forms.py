@@ -2,7 +2,10 @@
 import torch
 
 from distributedpytorch_amd import ops
+from distributedpytorch_amd.nn.engine import Act, Context, ParamStore, Tape
+from distributedpytorch_amd.nn.layers import Mlp
 from tests import train_ops_cases as cases
+from tests import train_ops_nets as nets
 from tests import train_ops_oracle as O
 
 # (n, h, w, c, groups): layouts without 16-byte vectors, small and large; with them, an image in one pass and in two
@@ -25,3 +28,33 @@ def check_dresidual_alone(case, act, dtype, device):
         ops.group_norm_bwd(dy.to(device), xd, gd, bd, groups, mean, rstd, dx, dg, db, act=act, y=mask, dresidual=dres)
         for k, got in enumerate((dx, dg, db, dres)):
             O.close(("dx", "dgamma", "dbeta", "dresidual")[k], got, want[k], err[k], dtype if k in (0, 3) else torch.float32)
+
+
+NARROW = [(16, 4, 10), (16, 1, 3), (512, 3, 2, 10), (24, 7, 1)]
+
+
+def check_narrow_mlp(widths, device):
+    """Hidden layers of fewer units than a 16-byte vector holds, against torch."""
+    torch.manual_seed(sum(widths))
+    store = ParamStore(device, torch.float32)
+    m = Mlp(store, "m", widths, "gelu")
+    store.finalize()
+    x, dy = torch.randn(9, widths[0]), torch.randn(9, widths[-1])
+    ctx = Context(store, True, Tape())
+    xa = Act(x.view(9, 1, 1, -1).to(device), True)
+    out = m(ctx, xa)
+    out.grad = torch.zeros_like(out.data)
+    out.grad[..., : widths[-1]] = dy.view(9, 1, 1, -1).to(device)
+    y = out.data[:, 0, 0, : widths[-1]].clone()
+    ctx.tape.backward()
+    p = {s.name: store.get_logical(s).cpu().double().requires_grad_() for s in store.params}
+    xd = x.double().requires_grad_()
+    h = xd
+    for i in range(len(widths) - 1):
+        h = torch.nn.functional.linear(h if i == 0 else torch.nn.functional.gelu(h), p[f"m.{2 * i}.weight"], p[f"m.{2 * i}.bias"])
+    h.backward(dy.double())
+    # three products of at most 512 + 16 roundings and 32 elementwise ones each, forward and back, in norm over random data
+    tol = 6 * 560 * O.E
+    assert nets.rel(y, h) <= tol and nets.rel(xa.grad.view(9, -1), xd.grad) <= tol
+    for s in store.params:
+        assert nets.rel(store.storage_to_logical(s, store.gview(s)), p[s.name].grad) <= tol, s.name
