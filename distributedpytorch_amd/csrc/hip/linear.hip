@@ -89,8 +89,13 @@ __global__ void __launch_bounds__(256) lin_colsum_kernel(const T* __restrict__ x
   }
 }
 __global__ void __launch_bounds__(256) lin_colsum_join_kernel(const float* slab, int parts, int cols, int accumulate, float* out) {
-  lin_join_sums(slab, parts, cols, accumulate, out, blockIdx.x);
+  for (int b = blockIdx.x; b * 16LL < cols; b += gridDim.x) {
+    lin_join_sums(slab, parts, cols, accumulate, out, b);
+    __syncthreads();
+  }
 }
+// (a launch has fewer than 2^32 threads)
+static int lin_join_grid(int cols) { return (int)min((cols + 15LL) / 16, 65536LL); }
 
 template <typename T>
 static void lin_colsum(const LinCall& c, hipStream_t s) {
@@ -102,7 +107,7 @@ static void lin_colsum(const LinCall& c, hipStream_t s) {
   const dim3 grid((wide + lanes - 1) / lanes, c.db_splits);
   if (vec) lin_colsum_kernel<T, true><<<grid, 256, 0, s>>>((const T*)c.src_a, c.src_lda, rows, cols, per, lanes, c.db_slab);
   else lin_colsum_kernel<T, false><<<grid, 256, 0, s>>>((const T*)c.src_a, c.src_lda, rows, cols, per, lanes, c.db_slab);
-  lin_colsum_join_kernel<<<(cols + 15) / 16, 256, 0, s>>>(c.db_slab, c.db_splits, cols, c.p.accumulate, c.db);
+  lin_colsum_join_kernel<<<lin_join_grid(cols), 256, 0, s>>>(c.db_slab, c.db_splits, cols, c.p.accumulate, c.db);
 }
 
 // ---- few rows (fprop, M <= 16 * MT): the weights are read once, straight into registers ------------------------------------
@@ -215,7 +220,7 @@ DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
   }
   if (rc || !c.db) return rc;
   if (c.p.sums) {
-    if (c.p.splits == 1 && c.p.db) lin_colsum_join_kernel<<<(c.a_cols + 15) / 16, 256, 0, s>>>(c.p.sums, c.p.takers, c.a_cols, c.p.accumulate, c.db);
+    if (c.p.splits == 1 && c.p.db) lin_colsum_join_kernel<<<lin_join_grid(c.a_cols), 256, 0, s>>>(c.p.sums, c.p.takers, c.a_cols, c.p.accumulate, c.db);
   } else if (c.f32) lin_colsum<float>(c, s); else lin_colsum<bf16_t>(c, s);
   return dpa_launch_rc();
 }

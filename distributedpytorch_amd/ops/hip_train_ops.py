@@ -73,9 +73,23 @@ def _gn_plan(n, hw, c, cg, v, bwd):
     Few images make too few blocks: then the chunk is as narrow as it goes (4 images of 28 x 28 x 512: 7.1 forward and 13.2
     backward, 10.5 and 19.1 in 128 bytes), and a large image goes through two passes (4 of 56 x 56 x 256: 15.5 and 26.8, one
     pass 19.9 and 28.5; with 16 images 26.3 and 75.7, one pass 20.4 and 46.8).
+    A launch has fewer than 2^32 threads: more chunks of images than that take the kernels for any layout, which loop over images.
     Without 16-byte vectors a lane holds one channel; up to 16 pixels a lane that is faster than the kernels for any layout
     (64 images of 22 x 22 x 90, fp32: 12.6 forward and 16.1 backward, 17.2 and 24.4), with 52 it is not (31 x 31 x 90, bf16 with
     a residual: 33.1 and 63.4, 24.7 and 44.7)."""
+    plan = _gn_chunks(n, hw, c, cg, v, bwd) if v else None
+    if plan is not None:
+        way, threads, w, _, _, s, _ = plan
+        if n * s * (c // (w if way == _LONE else w * v)) * threads < 1 << 32:
+            return plan
+    blocks = n * _cdiv(c, 64)
+    s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64), min(_cdiv(hw, 2048), 65535))          # (512 pixels a thread)
+    pps = _cdiv(hw, s)
+    return _ANY, 256, 1, 1, 1, _cdiv(hw, pps), pps
+
+
+def _gn_chunks(n, hw, c, cg, v, bwd):
+    """The plan of the kernels that own chunks of an image's channels, or None where none of them takes it."""
     if v > 1:
         unit = cg * v // math.gcd(cg, v) // v          # vectors of the smallest chunk of whole groups
         total = c // v
@@ -96,16 +110,12 @@ def _gn_plan(n, hw, c, cg, v, bwd):
             pps = rows * r * (max(1, min(n * _cdiv(hw, rows * r) * (total // w) // 1024, 32)) if bwd else 1)
             if hw <= 2048 * pps:
                 return _TWO, 512, w, rows, r, _cdiv(hw, pps), pps
-    if v:
-        for want in (32, 16, 1) if n * c >= 8192 else (1,):
-            for threads, r in ((256, 4), (512, 16)):
-                for w in range(cg, min(c, threads) + 1, cg):
-                    if c % w == 0 and (w >= want or w == c) and hw <= threads // w * r:
-                        return _LONE, threads, w, threads // w, r, 1, hw
-    blocks = n * _cdiv(c, 64)
-    s = max(1, min(_cdiv(hw, 16), 2048 // max(blocks, 1), 64), min(_cdiv(hw, 2048), 65535))          # (512 pixels a thread)
-    pps = _cdiv(hw, s)
-    return _ANY, 256, 1, 1, 1, _cdiv(hw, pps), pps
+    for want in (32, 16, 1) if n * c >= 8192 else (1,):
+        for threads, r in ((256, 4), (512, 16)):
+            for w in range(cg, min(c, threads) + 1, cg):
+                if c % w == 0 and (w >= want or w == c) and hw <= threads // w * r:
+                    return _LONE, threads, w, threads // w, r, 1, hw
+    return None
 
 
 def _gn(x, groups, spans, vecs, grads, bwd, a, eps):
@@ -208,8 +218,8 @@ def _linear(stream, epi, t_a, a, t_b, b, rows, cols, k, vec, act=0, out=checks.N
     at_a, lda, at_b, ldb = src_a, src_lda, src_b, src_ldb
     parts = 3 if f32 else 1
     need = ld_a = ld_b = a_part = b_part = pack_a = pack_b = ws = sums = db_out = db_slab = takers = db_splits = 0
-    if epi == _FPROP and rows <= (64 if f32 else 32) and ok_a and ok_b and not (k * es) & 15:
-        # (32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
+    if epi == _FPROP and rows <= (64 if f32 else 32) and cols < 1 << 27 and ok_a and ok_b and not (k * es) & 15:
+        # (a launch has fewer than 2^32 threads, 32 for a column; 32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
         tile, splits = -1, 1
     else:
         tile, splits = _plan(rows, cols, k, f32)

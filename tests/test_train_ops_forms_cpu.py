@@ -38,3 +38,16 @@ def test_widths_and_channels_are_refused():
     store.finalize()
     with pytest.raises(ValueError, match="m.weight takes 16 channels"):
         m(Context(store, True, Tape()), Act(torch.zeros(2, 1, 1, 24), False))
+
+
+def test_no_group_norm_plan_is_larger_than_a_launch():
+    """A launch has fewer than 2^32 threads; the kernels for any layout loop over images instead."""
+    from distributedpytorch_amd.ops import hip_train_ops as h
+    for n in (1 << 22, (1 << 23) + 1, 1 << 24, (1 << 27) + 5):
+        for c, groups in ((8, 1), (8, 8), (64, 64), (512, 32), (30, 3), (7, 7)):
+            for hw in (1, 4, 9):
+                for v in (8, 4, 1, 0):
+                    if v < 2 or c % v == 0:
+                        for bwd in (0, 1):
+                            way, threads, w, _, _, s, _ = h._gn_plan(n, hw, c, c // groups, v, bwd)
+                            assert way == h._ANY or n * s * (c // (w if way == h._LONE else w * v)) * threads < 1 << 32
