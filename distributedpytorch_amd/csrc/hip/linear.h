@@ -24,7 +24,7 @@ struct LinParams {
   float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns), or null
   float* db;                            // [rows] what they are joined into, the bias gradient; null: sums is it
   long long ld_add, ld_pre, ld_out, ld_z;
-  int rows, cols, K, parts, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
+  int rows, cols, K, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
 };
 
 // What a call hands over besides: the operands as they are, what they are packed into first (ld 0: nothing), the bias gradient.
@@ -34,7 +34,7 @@ struct LinCall {
   void *pack_a, *pack_b;
   float *db, *db_slab;
   long long src_lda, src_ldb;
-  int a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, vec_a, vec_b, db_splits, epi, tile, f32;
+  int a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, vec_a, vec_b, db_splits, epi, tile, f32;      // (f32: the operands are)
 };
 
 enum : int { EPI_FPROP = 0, EPI_DGRAD = 1, EPI_WGRAD = 2 };
@@ -174,19 +174,21 @@ __device__ __forceinline__ bf16x8 lin_fragment(const char* t, int u, int ks, int
 // all but this wave's newest N pieces have landed and its LDS reads are done; behind the barrier, everyone's
 template <int N> __device__ __forceinline__ void lin_sync() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// a kernel that can make the row sums on its way (the 256 x 256 tile has no registers for them)
+// a kernel that can make the row sums on its way (the 256 x 256 tile has no registers for them, and one part a step would count
+// the rows of fp32 operands once for each pass)
 template <int MT, int EPI> constexpr bool lin_sums() { return EPI == EPI_WGRAD && MT <= 4; }
 
 // The blocks are persistent and see ONE stream of K steps across their tiles, S of them in LDS: while step s is multiplied, the
 // steps behind it land, and step s + S is requested as soon as the buffer of step s is free, also when it belongs to the next
 // tile, so the epilogue of a tile runs under the first loads of the next.
+// PARTS: of the operands, 1 (bf16) or 3 (fp32).  P: the parts of them in a step.
 // P = 1: a step has four phases, each the matrix instructions of half the wave's rows and half the step; a phase first reads
 // the fragments of the NEXT phase from LDS.  The barrier stands before the last phase: behind it everyone's reads of the
 // buffer are done (registers hold what is left to multiply) and everyone's pieces of step s + 1 have landed.
 // P = 3: all three parts of both operands, each fragment read once for the six products of fp32 (P = 1 on parts walks over
 // them six times).  Half the LDS and DMA traffic, for tiles of which a CU has no second one to hide it behind; the larger
 // tile has no registers for it.  The fragments of step s + 1 are read while step s is multiplied.
-template <typename T, int WM, int WN, int MT, int NT, int S, int P, int EPI>
+template <typename T, int PARTS, int WM, int WN, int MT, int NT, int S, int P, int EPI>
 __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mfma_kernel(LinParams p) {
   constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
   constexpr int BM = WM * MT * 16, BN = WN * NT * 16, NW = WM * WN, H = MT / 2, BK = P == 1 ? 64 : 32;
@@ -196,7 +198,9 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int tm = (p.rows + BM - 1) / BM, tn = (p.cols + BN - 1) / BN, tiles = tm * tn, jobs = tiles * p.splits;
-  const int ksteps = (p.K + BK - 1) / BK, passes = P == 1 && p.parts == 3 ? 6 : 1, total = ksteps * passes, per = (total + p.splits - 1) / p.splits;
+  constexpr int passes = P < PARTS ? 6 : 1;
+  static_assert(P <= PARTS && !(passes > 1 && lin_sums<MT, EPI>()), "parts");
+  const int ksteps = (p.K + BK - 1) / BK, total = ksteps * passes, per = (total + p.splits - 1) / p.splits;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
 
   // blocks of one XCD get neighbouring tiles: panels of 8 tile rows, walked column by column
@@ -519,7 +523,7 @@ __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p, int main) {
 }
 
 // Blocks on the chip at a time: a multiple of 8 where a launch has several rounds (xcd_remap).
-template <typename T, int WM, int WN, int MT, int NT, int S, int P, int EPI>
+template <typename T, int PARTS, int WM, int WN, int MT, int NT, int S, int P, int EPI>
 static int lin_run(const LinParams& p, hipStream_t s) {
   constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
   constexpr int lds = S * (BM + BN) * (P == 1 ? 128 : 192), residents = 160 * 1024 / lds;
@@ -530,13 +534,13 @@ static int lin_run(const LinParams& p, hipStream_t s) {
     int dev = 0;
     if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
     if (dev >= 64 || !done[dev].load(std::memory_order_relaxed)) {
-      const hipError_t e = hipFuncSetAttribute((const void*)lin_mfma_kernel<T, WM, WN, MT, NT, S, P, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      const hipError_t e = hipFuncSetAttribute((const void*)lin_mfma_kernel<T, PARTS, WM, WN, MT, NT, S, P, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e) return (int)e;
       if (dev < 64) done[dev].store(1, std::memory_order_relaxed);
     }
   }
   const int grid = (int)(jobs < 256 * residents ? jobs : 256 * residents);
-  lin_mfma_kernel<T, WM, WN, MT, NT, S, P, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
+  lin_mfma_kernel<T, PARTS, WM, WN, MT, NT, S, P, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
   if (p.splits > 1) {
     const int main = dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256);
     lin_join_kernel<T, EPI><<<main + (p.sums ? (p.rows + 15) / 16 : 0), 256, 0, s>>>(p, main);
@@ -544,15 +548,20 @@ static int lin_run(const LinParams& p, hipStream_t s) {
   return dpa_launch_rc();
 }
 
-template <typename T, int EPI>
+template <typename T, int PARTS, int EPI>
 static int lin_tile(const LinParams& p, int tile, hipStream_t s) {
-  switch (tile) {
-    case 0: return lin_run<T, 2, 4, 8, 4, 2, 1, EPI>(p, s);      // 256 x 256, 8 waves
-    case 1: return lin_run<T, 2, 2, 4, 4, 2, 1, EPI>(p, s);      // 128 x 128, 4 waves, two blocks a CU
-    case 2: return lin_run<T, 2, 2, 4, 4, 4, 1, EPI>(p, s);      // 128 x 128, four steps in LDS
-    case 3: return lin_run<T, 2, 2, 2, 2, 4, 1, EPI>(p, s);      // 64 x 64, two blocks a CU
-    case 4: if constexpr (sizeof(T) == 4) return lin_run<T, 2, 2, 4, 4, 3, 3, EPI>(p, s); break;      // 128 x 128, three parts at once
-    case 5: if constexpr (sizeof(T) == 4) return lin_run<T, 2, 2, 2, 2, 4, 3, EPI>(p, s); break;      // 64 x 64, three parts at once
+  if (tile == 0) return lin_run<T, PARTS, 2, 4, 8, 4, 2, 1, EPI>(p, s);      // 256 x 256, 8 waves
+  if constexpr (PARTS == 1) {
+    switch (tile) {
+      case 1: return lin_run<T, 1, 2, 2, 4, 4, 2, 1, EPI>(p, s);      // 128 x 128, 4 waves, two blocks a CU
+      case 2: return lin_run<T, 1, 2, 2, 4, 4, 4, 1, EPI>(p, s);      // 128 x 128, four steps in LDS
+      case 3: return lin_run<T, 1, 2, 2, 2, 2, 4, 1, EPI>(p, s);      // 64 x 64, two blocks a CU
+    }
+  } else {
+    switch (tile) {
+      case 4: return lin_run<T, 3, 2, 2, 4, 4, 3, 3, EPI>(p, s);      // 128 x 128, three parts at once
+      case 5: return lin_run<T, 3, 2, 2, 2, 2, 4, 3, EPI>(p, s);      // 64 x 64, three parts at once
+    }
   }
   return (int)hipErrorInvalidValue;
 }

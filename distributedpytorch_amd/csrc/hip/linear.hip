@@ -1,9 +1,9 @@
 // Entry points of the linear products (linear.h), the operand packing and the bias gradient.
 #include "linear.h"
 
-int lin_fprop(const LinParams& p, int tile, hipStream_t s);
-int lin_dgrad(const LinParams& p, int tile, hipStream_t s);
-int lin_wgrad(const LinParams& p, int tile, hipStream_t s);
+int lin_fprop(const LinParams& p, int tile, bool f32, hipStream_t s);
+int lin_dgrad(const LinParams& p, int tile, bool f32, hipStream_t s);
+int lin_wgrad(const LinParams& p, int tile, bool f32, hipStream_t s);
 
 // ---- operands that the DMA cannot take as they are -----------------------------------------------------------------------
 // fp32 matrices become their three bf16 parts, bf16 matrices with odd rows or addresses a copy with rows of a multiple of 8;
@@ -214,9 +214,9 @@ DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
   }
   int rc = (int)hipErrorInvalidValue;
   switch (c.epi) {
-    case EPI_FPROP: rc = c.tile >= 0 ? lin_fprop(c.p, c.tile, s) : c.f32 ? lin_rows<float>(c.p, s) : lin_rows<bf16_t>(c.p, s); break;
-    case EPI_DGRAD: rc = lin_dgrad(c.p, c.tile, s); break;
-    case EPI_WGRAD: rc = lin_wgrad(c.p, c.tile, s); break;
+    case EPI_FPROP: rc = c.tile >= 0 ? lin_fprop(c.p, c.tile, c.f32, s) : c.f32 ? lin_rows<float>(c.p, s) : lin_rows<bf16_t>(c.p, s); break;
+    case EPI_DGRAD: rc = lin_dgrad(c.p, c.tile, c.f32, s); break;
+    case EPI_WGRAD: rc = lin_wgrad(c.p, c.tile, c.f32, s); break;
   }
   if (rc || !c.db) return rc;
   if (c.p.sums) {

@@ -22,9 +22,9 @@ _F32 = torch.float32
 _GN_PARAMS = struct.Struct("@15Q7q13if")
 
 
-# LinCall of csrc/hip/linear.h: operands and their strides; bias, addend, pre, out, preact, workspaces; strides; ten integers; the
+# LinCall of csrc/hip/linear.h: operands and their strides; bias, addend, pre, out, preact, workspaces; strides; nine integers; the
 # operands as they are and what they are packed into, the bias gradient and its slab; strides; twelve integers
-_LIN_CALL = struct.Struct("@2Q4q8Q4q10i6Q2q12i")
+_LIN_CALL = struct.Struct("@2Q4q8Q4q9i6Q2q12i")
 
 
 _loaded = []
@@ -263,7 +263,7 @@ def _linear(stream, epi, t_a, a, t_b, b, rows, cols, k, vec, act=0, out=checks.N
             db_slab += at
     _lib().dpa_linear(_LIN_CALL.pack(
         at_a, at_b, lda, ldb, a_part, b_part, bias, addend[0], pre[0], out[0], preact[0], ws, sums, db_out,
-        addend[1], pre[1], out[1], preact[1], rows, cols, k, parts, splits, accumulate, act, vec, bias_vec, takers,
+        addend[1], pre[1], out[1], preact[1], rows, cols, k, splits, accumulate, act, vec, bias_vec, takers,
         src_a, src_b, pack_a, pack_b, db, db_slab, src_lda, src_ldb,
         a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, ok_a, ok_b, db_splits, epi, tile, f32), stream)
 
