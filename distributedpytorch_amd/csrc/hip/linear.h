@@ -24,16 +24,16 @@ struct LinParams {
   float* sums;                          // [splits * takers][rows] partial sums of a's rows (dy's columns), or null
   float* db;                            // [rows] what they are joined into, the bias gradient; null: sums is it
   long long ld_add, ld_pre, ld_out, ld_z;
+  const void *src_a, *src_b;            // the operands as the caller has them
+  long long src_lda, src_ldb;
   int rows, cols, K, splits, accumulate, act, vec, bias_vec, takers;      // vec: every matrix of the epilogue takes 16-byte access
 };
 
 // What a call hands over besides: the operands as they are, what they are packed into first (ld 0: nothing), the bias gradient.
 struct LinCall {
   LinParams p;
-  const void *src_a, *src_b;
   void *pack_a, *pack_b;
   float *db, *db_slab;
-  long long src_lda, src_ldb;
   int a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, vec_a, vec_b, db_splits, epi, tile, f32;      // (f32: the operands are)
 };
 
@@ -91,8 +91,31 @@ __device__ __forceinline__ void lin_extra(const LinParams& p, int i, int j, int 
   if (EPI == EPI_DGRAD && ACT != ACT_NONE) x.pre.template load<VEC>((const T*)p.pre + i * p.ld_pre + j, n);
 }
 
-template <typename T, int EPI, int ACT, bool VEC>
+// An infinity is one part and two zeros, so its products with the other operand's parts hold infinity times zero, and differences of
+// infinities: NaN where fp32 gives an infinity.  Elements that came out as NaN are computed again from the operands themselves.
+template <int EPI>
+__device__ __forceinline__ void lin_again(const LinParams& p, int i, int j, int n, float (&v)[8]) {
+  constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
+  unsigned bad = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bad |= (unsigned)(v[e] != v[e]) << e;
+  bad &= (1u << n) - 1;
+  while (bad) {
+    const int at = __builtin_ctz(bad);
+    bad &= bad - 1;
+    const float* a = (const float*)p.src_a + (AT ? i : i * p.src_lda);
+    const float* b = (const float*)p.src_b + (BT ? j + at : (j + at) * p.src_ldb);
+    float s = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < p.K && s == s; ++k) s = fmaf(a[AT ? k * p.src_lda : k], b[BT ? k * p.src_ldb : k], s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e == at ? s : v[e];
+  }
+}
+
+template <typename T, int PARTS, int EPI, int ACT, bool VEC>
 __device__ __forceinline__ void lin_finish(const LinParams& p, int i, int j, int n, const LinExtra<T>& x, const Lin8<float>& bias, float (&v)[8]) {
+  if constexpr (PARTS == 3) lin_again<EPI>(p, i, j, n, v);
   if (EPI == EPI_FPROP) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias.get(e);
@@ -470,7 +493,7 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
                 }
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
-                  if (where(i, k, gi, gj)) lin_finish<T, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), x[k], bias[k], v[k]);
+                  if (where(i, k, gi, gj)) lin_finish<T, PARTS, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), x[k], bias[k], v[k]);
               });
       });
     }
@@ -497,7 +520,7 @@ __device__ __forceinline__ void lin_join_sums(const float* __restrict__ slab, in
 
 // joins the partial products of a split reduction in a fixed order and applies the epilogue; the blocks behind the first `main`
 // ones join the bias gradient
-template <typename T, int EPI>
+template <typename T, int PARTS, int EPI>
 __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p, int main) {
   if ((int)blockIdx.x >= main) return lin_join_sums(p.sums, p.splits * p.takers, p.rows, p.accumulate, p.db, blockIdx.x - main);
   const int groups = (p.cols + 7) / 8;
@@ -517,7 +540,7 @@ __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p, int main) {
     lin_by_kind<EPI>(p, [&](auto act, auto vec) {
       LinExtra<T> x;
       lin_extra<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x);
-      lin_finish<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x, lin_bias<EPI>(p, j, p.bias_vec), v);
+      lin_finish<T, PARTS, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x, lin_bias<EPI>(p, j, p.bias_vec), v);
     });
   }
 }
@@ -543,7 +566,7 @@ static int lin_run(const LinParams& p, hipStream_t s) {
   lin_mfma_kernel<T, PARTS, WM, WN, MT, NT, S, P, EPI><<<grid, WM * WN * 64, lds, s>>>(p);
   if (p.splits > 1) {
     const int main = dpa_grid((long long)p.rows * ((p.cols + 7) / 8), 256);
-    lin_join_kernel<T, EPI><<<main + (p.sums ? (p.rows + 15) / 16 : 0), 256, 0, s>>>(p, main);
+    lin_join_kernel<T, PARTS, EPI><<<main + (p.sums ? (p.rows + 15) / 16 : 0), 256, 0, s>>>(p, main);
   }
   return dpa_launch_rc();
 }

@@ -7,8 +7,7 @@ int lin_wgrad(const LinParams& p, int tile, bool f32, hipStream_t s);
 
 // ---- operands that the DMA cannot take as they are -----------------------------------------------------------------------
 // fp32 matrices become their three bf16 parts, bf16 matrices with odd rows or addresses a copy with rows of a multiple of 8;
-// the columns behind the last one are zeros.  (An infinity has no remainder: its other parts are zero, and its product with
-// a number whose parts differ in sign is NaN where fp32 gives an infinity.)
+// the columns behind the last one are zeros.  (An infinity has no remainder, its other parts are zero: lin_again.)
 struct LinPack { const void* src; bf16_t* dst; long long ld; int rows, cols, ldd, vec; };
 
 template <typename T>
@@ -105,8 +104,8 @@ static void lin_colsum(const LinCall& c, hipStream_t s) {
   int lanes = 64;
   while (lanes > 4 && lanes / 2 >= wide) lanes /= 2;
   const dim3 grid((wide + lanes - 1) / lanes, c.db_splits);
-  if (vec) lin_colsum_kernel<T, true><<<grid, 256, 0, s>>>((const T*)c.src_a, c.src_lda, rows, cols, per, lanes, c.db_slab);
-  else lin_colsum_kernel<T, false><<<grid, 256, 0, s>>>((const T*)c.src_a, c.src_lda, rows, cols, per, lanes, c.db_slab);
+  if (vec) lin_colsum_kernel<T, true><<<grid, 256, 0, s>>>((const T*)c.p.src_a, c.p.src_lda, rows, cols, per, lanes, c.db_slab);
+  else lin_colsum_kernel<T, false><<<grid, 256, 0, s>>>((const T*)c.p.src_a, c.p.src_lda, rows, cols, per, lanes, c.db_slab);
   lin_colsum_join_kernel<<<lin_join_grid(cols), 256, 0, s>>>(c.db_slab, c.db_splits, cols, c.p.accumulate, c.db);
 }
 
@@ -204,7 +203,7 @@ DPA_API int dpa_lin_params_size() { return (int)sizeof(LinCall); }
 DPA_API int dpa_linear(const LinCall* call, hipStream_t s) {
   const LinCall& c = *call;
   if (c.ld_a || c.ld_b) {
-    LinPack a{c.src_a, (bf16_t*)c.pack_a, c.src_lda, c.a_rows, c.a_cols, c.ld_a, c.vec_a}, b{c.src_b, (bf16_t*)c.pack_b, c.src_ldb, c.b_rows, c.b_cols, c.ld_b, c.vec_b};
+    LinPack a{c.p.src_a, (bf16_t*)c.pack_a, c.p.src_lda, c.a_rows, c.a_cols, c.ld_a, c.vec_a}, b{c.p.src_b, (bf16_t*)c.pack_b, c.p.src_ldb, c.b_rows, c.b_cols, c.ld_b, c.vec_b};
     if (!c.ld_a) a = b;
     const long long na = (long long)a.rows * (a.ldd / 8), nb = c.ld_a && c.ld_b ? (long long)b.rows * (b.ldd / 8) : 0;
     const dim3 grid(dpa_grid(na > nb ? na : nb, 256), nb ? 2 : 1);

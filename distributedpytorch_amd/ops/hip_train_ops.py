@@ -22,9 +22,9 @@ _F32 = torch.float32
 _GN_PARAMS = struct.Struct("@15Q7q13if")
 
 
-# LinCall of csrc/hip/linear.h: operands and their strides; bias, addend, pre, out, preact, workspaces; strides; nine integers; the
-# operands as they are and what they are packed into, the bias gradient and its slab; strides; twelve integers
-_LIN_CALL = struct.Struct("@2Q4q8Q4q9i6Q2q12i")
+# LinCall of csrc/hip/linear.h: operands and their strides; bias, addend, pre, out, preact, workspaces; strides; the operands as they
+# are and their strides; nine integers; what the operands are packed into, the bias gradient and its slab; twelve integers
+_LIN_CALL = struct.Struct("@2Q4q8Q4q2Q2q9i4Q12i")
 
 
 _loaded = []
@@ -263,8 +263,8 @@ def _linear(stream, epi, t_a, a, t_b, b, rows, cols, k, vec, act=0, out=checks.N
             db_slab += at
     _lib().dpa_linear(_LIN_CALL.pack(
         at_a, at_b, lda, ldb, a_part, b_part, bias, addend[0], pre[0], out[0], preact[0], ws, sums, db_out,
-        addend[1], pre[1], out[1], preact[1], rows, cols, k, splits, accumulate, act, vec, bias_vec, takers,
-        src_a, src_b, pack_a, pack_b, db, db_slab, src_lda, src_ldb,
+        addend[1], pre[1], out[1], preact[1], src_a, src_b, src_lda, src_ldb, rows, cols, k, splits, accumulate, act, vec,
+        bias_vec, takers, pack_a, pack_b, db, db_slab,
         a_rows, a_cols, b_rows, b_cols, ld_a, ld_b, ok_a, ok_b, db_splits, epi, tile, f32), stream)
 
 

@@ -63,3 +63,9 @@ def test_more_columns_than_a_launch_of_the_kernel_for_few_rows_has():
         want, err = O.product(x.cpu(), w[sl].cpu())
         O.close("y", y[:, sl], want, err, torch.bfloat16)
     assert torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("case", forms.INF, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinities_in_a_product(case, dtype):
+    forms.check_infinities(case, dtype, "cuda")

@@ -51,3 +51,9 @@ def test_no_group_norm_plan_is_larger_than_a_launch():
                         for bwd in (0, 1):
                             way, threads, w, _, _, s, _ = h._gn_plan(n, hw, c, c // groups, v, bwd)
                             assert way == h._ANY or n * s * (c // (w if way == h._LONE else w * v)) * threads < 1 << 32
+
+
+@pytest.mark.parametrize("case", forms.INF[:3], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinities_in_a_product(case, dtype):
+    forms.check_infinities(case, dtype, "cpu")

@@ -58,3 +58,39 @@ def check_narrow_mlp(widths, device):
     assert nets.rel(y, h) <= tol and nets.rel(xa.grad.view(9, -1), xd.grad) <= tol
     for s in store.params:
         assert nets.rel(store.storage_to_logical(s, store.gview(s)), p[s.name].grad) <= tol, s.name
+
+
+# (rows, out, in): the kernel for few rows and the one behind its bound, tiles and splits of every kind
+INF = [(64, 40, 72), (65, 40, 72), (300, 260, 264), (1000, 520, 4100), (3500, 3700, 24)]
+
+
+def check_infinities(case, dtype, device):
+    """Infinities in an operand: an infinity of the right sign, or NaN where the formula in fp32 has one, whatever kernel takes the sizes."""
+    m, n, k = case
+    gen = torch.Generator().manual_seed(m + n + k)
+    x, w, dy = (torch.randn(*s, generator=gen).to(dtype) for s in ((m, k), (n, k), (m, n)))
+    # numbers of one bf16 part beside those of three, and zeros: infinity times zero is NaN
+    for t in (x, w, dy):
+        t[:, 1::5] = t[:, 1::5].sign()
+        t[::7, 3::5] = 0
+    x[5, 3], x[9, 2], x[9, 7], x[m - 1, k - 1] = float("inf"), float("inf"), -float("inf"), -float("inf")
+    w[11, 6] = -float("inf")
+    dy[7, 4], dy[2, 0], dy[m - 1, 9] = float("inf"), -float("inf"), float("nan")
+    xd, wd, dyd = x.to(device), w.to(device), dy.to(device)
+
+    def nan(*s, dt=dtype):
+        return torch.full(s, float("nan"), dtype=dt, device=device)
+    for act in ("none", "relu"):
+        y = nan(m, n)
+        ops.linear_fprop(xd, wd, y, act=act)
+        want, err = O.product(x, w)
+        O.close("y", y, torch.where(want.isnan(), want, O.phi(want, act)[0]), err, dtype)
+    dx, add = nan(m, k), torch.randn(m, k, generator=gen).to(dtype)
+    ops.linear_dgrad(dyd, wd, dx, addend=add.to(device))
+    want, err = O.product(dy, w.t())
+    O.close("dx", dx, want + add.to(O.D), err + 2 * O.E * (want.abs() + add.to(O.D).abs()), dtype)
+    dw, db = nan(n, k, dt=torch.float32), nan(n, dt=torch.float32)
+    ops.linear_wgrad(dyd, xd, dw, db)
+    want, err = O.product(dy.t(), x.t())
+    O.close("dw", dw, want, err)
+    O.close("db", db, dy.to(O.D).sum(0), (m + 8) * O.E * dy.to(O.D).abs().sum(0))
