@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from distributedpytorch_amd import ops
+from tests import train_ops_cases as cases
 from tests import train_ops_forms as forms
 from tests import train_ops_oracle as O
 
@@ -69,3 +70,15 @@ def test_more_columns_than_a_launch_of_the_kernel_for_few_rows_has():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_infinities_in_a_product(case, dtype):
     forms.check_infinities(case, dtype, "cuda")
+
+
+@pytest.mark.parametrize("case", forms.GN, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_group_norm(case, dtype):
+    cases.check_group_norm(case, dtype, "cuda")
+
+
+@pytest.mark.parametrize("case", forms.LINEAR, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear(case, dtype):
+    cases.check_linear(case, dtype, "cuda")

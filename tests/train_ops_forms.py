@@ -30,6 +30,23 @@ def check_dresidual_alone(case, act, dtype, device):
             O.close(("dx", "dgamma", "dbeta", "dresidual")[k], got, want[k], err[k], dtype if k in (0, 3) else torch.float32)
 
 
+# What the plans choose beyond the cases of train_ops_cases: images of 2 to 13 vectors a thread, in groups of whole vectors and of parts
+# of them, layers of 28 x 28 x 512 and 31 x 31 x 512
+GN = [(1, 1, 86, 24, 8, "relu", True, ""), (1, 7, 37, 4, 4, "silu", True, ""), (1, 9, 2, 824, 4, "gelu", True, ""), (1, 113, 2, 36, 4, "relu", False, ""),
+      (1, 7, 11, 104, 1, "silu", True, "inplace"), (1, 1, 17, 1544, 8, "relu", True, ""), (1, 3, 43, 216, 1, "relu", True, "inplace"),
+      (1, 9, 2, 764, 4, "silu", False, ""), (1, 1, 66, 208, 1, "gelu", True, ""), (1, 14, 3, 1144, 8, "silu", True, "inplace"),
+      (1, 2, 158, 168, 1, "relu", True, ""), (1, 5, 6, 788, 4, "none", True, ""), (1, 108, 1, 232, 1, "gelu", False, ""),
+      (2, 3, 43, 216, 1, "gelu", True, "slice"), (16, 28, 28, 512, 32, "relu", True, ""), (16, 31, 31, 512, 32, "silu", True, "")]
+
+# (rows, out, in, act, addend, extra), as train_ops_cases.LINEAR: every tile, split and way to the bias gradient in each direction
+LINEAR = [(29, 200, 264, "gelu", True, ""), (130, 300, 2100, "relu", True, ""), (130, 2100, 300, "gelu", False, "accumulate"),
+          (1500, 1500, 320, "silu", True, ""), (1500, 328, 1501, "gelu", True, ""), (2100, 2200, 320, "relu", False, ""), (2101, 320, 2199, "silu", False, ""),
+          (1000, 520, 4100, "gelu", True, "accumulate"), (600, 4104, 1000, "relu", True, "slice"), (4200, 600, 1000, "none", True, "accumulate"),
+          (1100, 1100, 1050, "silu", False, "accumulate"), (1100, 1700, 1600, "relu", False, ""), (1101, 2101, 2200, "gelu", True, "accumulate"),
+          (1700, 1600, 264, "gelu", True, ""), (1700, 264, 1600, "relu", True, "slice"), (1000, 1600, 600, "silu", True, ""), (300, 1700, 1600, "none", False, "accumulate"),
+          (5000, 40, 1600, "none", False, ""), (3701, 3499, 393, "gelu", True, ""), (3704, 392, 3504, "silu", True, "slice"), (392, 3704, 3504, "relu", False, ""),
+          (401, 3701, 3499, "none", False, "accumulate")]
+
 NARROW = [(16, 4, 10), (16, 1, 3), (512, 3, 2, 10), (24, 7, 1)]
 
 
