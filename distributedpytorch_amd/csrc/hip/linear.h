@@ -582,8 +582,8 @@ static int lin_tile(const LinParams& p, int tile, hipStream_t s) {
     }
   } else {
     switch (tile) {
-      case 4: return lin_run<T, 3, 2, 2, 4, 4, 3, 3, EPI>(p, s);      // 128 x 128, three parts at once
-      case 5: return lin_run<T, 3, 2, 2, 2, 2, 4, 3, EPI>(p, s);      // 64 x 64, three parts at once
+      case 4: return lin_run<T, 3, 2, 2, 4, 4, 3, 3, EPI>(p, s);      // 128 x 128, three parts at once, one block a CU
+      case 5: return lin_run<T, 3, 2, 2, 2, 2, 3, 3, EPI>(p, s);      // 64 x 64, three parts at once, two blocks a CU
     }
   }
   return (int)hipErrorInvalidValue;

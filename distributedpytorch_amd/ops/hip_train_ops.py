@@ -186,20 +186,24 @@ def _plan(rows, cols, k, f32):
         x 480: 80.6, 94.1); fp32 walks over K six times and has no such bound;
       128 x 128 from 140 tiles on (1433 x 1872 x 2640, 180 tiles: 36.6, 64 x 64 44.1; 715 x 560 x 1504, 30 tiles: 19, 13.4);
         two blocks a CU above 256 tiles (6306 x 1112 x 736: 22.6, one 28.8), four steps in LDS below (2048^3: 28.6, 30.4);
-      fp32 in tiles of 128 x 128 has one block a CU, so the last round has to be well filled (688 x 5688 x 888, 270 tiles:
-        88.7, 64 x 64 69.9), and a long reduction is split over it (976 x 744 x 5741: 84.8, 64 x 64 105.8);
+      fp32 in tiles of 128 x 128 has one block a CU, so the last round has to be well filled (688 x 5688 x 888, 270 tiles: 91.9,
+        64 x 64 82.3), and a long reduction is split over it (976 x 744 x 5741: 84 in five, 64 x 64 125 whole and 123 in two);
+        up to 512 elements a part 64 x 64 in one round needs no split and no launch to join it (1021 x 1000 x 2048: 44.0, 128 x
+        128 in four 45.8; 900 x 700 x 1600: 37.9, 51.7 in three);
       a split costs a pass over its partial products and pays from 512 elements a part on (3119 x 280 x 624: 9.6 whole, 15.8
         in two; 784 x 184 x 4670: 15.7 in six, 25 whole; 792 x 1424 x 6161 in 128 x 128: 36.8 in six, 57.8 in whole 64 x 64),
-        in fp32 with few tiles from 128 on (176 x 248 x 571: 13.6 in four, 16.8 whole)."""
+        in fp32 with few tiles from 128 on (176 x 248 x 571: 13.4 in four, 15.7 whole), as long as every part has a CU of its own: two
+        blocks share one's LDS traffic (256 x 1000 x 2048, 64 tiles: 28.2 in four, 30.5 in eight; 900 x 900 x 1400, 225 tiles:
+        44.0 whole, 52.5 in two; 700 x 700 x 2048, 121 tiles: 37.0 in two, 40.3 in four)."""
     if _cdiv(rows, 256) * _cdiv(cols, 256) >= 200 and (f32 or k >= 384):
         return 0, 1
     t128, t64 = _cdiv(rows, 128) * _cdiv(cols, 128), _cdiv(rows, 64) * _cdiv(cols, 64)
     if f32:
         if t128 >= 160 * _cdiv(t128, 256):
             return 4, 1
-        if 40 <= t128 <= 128 and k >= 1500:
+        if 40 <= t128 <= 128 and k >= 1500 and (t64 > 256 or k > 512 * (256 // t128)):
             return 4, min(256 // t128, k // 512)
-        return 5, max(1, min(512 // t64, k // (128 if t64 < 64 else 384), 16))
+        return 5, max(1, min(256 // t64, k // (128 if t64 < 64 else 384), 16))
     if k >= 4096 and 32 <= t128 < 200:
         return 1, min(512 // t128, k // 768, 16)
     if t128 >= 140:
