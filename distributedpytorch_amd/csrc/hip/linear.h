@@ -92,30 +92,27 @@ __device__ __forceinline__ void lin_extra(const LinParams& p, int i, int j, int 
 }
 
 // An infinity is one part and two zeros, so its products with the other operand's parts hold infinity times zero, and differences of
-// infinities: NaN where fp32 gives an infinity.  Elements that came out as NaN are computed again from the operands themselves.
+// infinities: NaN where fp32 gives an infinity.  Elements that came out as NaN are computed again from the operands themselves,
+// which are read where that happens: the kernels have no registers to keep their addresses in.
 template <int EPI>
-__device__ __forceinline__ void lin_again(const LinParams& p, int i, int j, int n, float (&v)[8]) {
+__device__ __forceinline__ float lin_again(bool bad, int i, int j, float v) {
   constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
-  unsigned bad = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) bad |= (unsigned)(v[e] != v[e]) << e;
-  bad &= (1u << n) - 1;
-  while (bad) {
-    const int at = __builtin_ctz(bad);
-    bad &= bad - 1;
-    const float* a = (const float*)p.src_a + (AT ? i : i * p.src_lda);
-    const float* b = (const float*)p.src_b + (BT ? j + at : (j + at) * p.src_ldb);
-    float s = 0.f;
-#pragma unroll 1
-    for (int k = 0; k < p.K && s == s; ++k) s = fmaf(a[AT ? k * p.src_lda : k], b[BT ? k * p.src_ldb : k], s);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e == at ? s : v[e];
-  }
+  auto p = (const __attribute__((address_space(4))) LinParams*)__builtin_amdgcn_kernarg_segment_ptr();      // (the first argument)
+  asm volatile("" : "+s"(p));
+  const float* a = (const float*)p->src_a + (AT ? i : i * p->src_lda);
+  const float* b = (const float*)p->src_b + (BT ? j : j * p->src_ldb);
+  const long long sa = AT ? p->src_lda : 1, sb = BT ? p->src_ldb : 1;
+  if (bad) v = 0.f;
+  for (int k = 0; k < p->K && __any(bad); ++k)
+    if (bad) {
+      v = fmaf(a[k * sa], b[k * sb], v);
+      bad = v == v;
+    }
+  return v;
 }
 
-template <typename T, int PARTS, int EPI, int ACT, bool VEC>
+template <typename T, int EPI, int ACT, bool VEC>
 __device__ __forceinline__ void lin_finish(const LinParams& p, int i, int j, int n, const LinExtra<T>& x, const Lin8<float>& bias, float (&v)[8]) {
-  if constexpr (PARTS == 3) lin_again<EPI>(p, i, j, n, v);
   if (EPI == EPI_FPROP) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += bias.get(e);
@@ -423,6 +420,40 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
       }
     }
 
+    if constexpr (PARTS == 3) {
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) some |= __builtin_isunordered(acc[i][j][0], acc[i][j][1]) | __builtin_isunordered(acc[i][j][2], acc[i][j][3]);
+      if (__any(some) && p.splits == 1) {          // (parts of a sum are joined first)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          unsigned bad = 0;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const f32x4 c = acc[i][j];
+            bad |= ((unsigned)(c[0] != c[0]) | (unsigned)(c[1] != c[1]) << 1 | (unsigned)(c[2] != c[2]) << 2 | (unsigned)(c[3] != c[3]) << 3) << (4 * j);
+          }
+          if (!__any(bad)) continue;
+          const int row = i0 + (wm * MT + i) * 16 + (lane & 15);
+#pragma unroll 1
+          for (int n = 0; n < NT * 4; ++n) {
+            const int col = j0 + (wn * NT + n / 4) * 16 + (lane >> 4) * 4 + (n & 3);
+            const bool now = (bad >> n & 1) && row < p.rows && col < p.cols;
+            if (!__any(now)) continue;
+            const float v = lin_again<EPI>(now, row, col, 0.f);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const int e = now && n / 4 == j ? n & 3 : 4;
+              const f32x4 c = acc[i][j];
+              acc[i][j] = (f32x4){e == 0 ? v : c[0], e == 1 ? v : c[1], e == 2 ? v : c[2], e == 3 ? v : c[3]};
+            }
+          }
+        }
+      }
+    }
+
     // ---- epilogue, from registers.  Neighbouring 16-column tiles trade quarters, so that a lane holds 8 columns of one row,
     // and the lanes are permuted so that four neighbouring ones hold 32 neighbouring columns: 64-byte requests instead of
     // 16-byte ones, each of which would take the address unit as long.
@@ -493,7 +524,7 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
                 }
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
-                  if (where(i, k, gi, gj)) lin_finish<T, PARTS, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), x[k], bias[k], v[k]);
+                  if (where(i, k, gi, gj)) lin_finish<T, EPI, ACT, VEC>(p, gi, gj, VEC ? 8 : min(8, p.cols - gj), x[k], bias[k], v[k]);
               });
       });
     }
@@ -537,10 +568,17 @@ __global__ void __launch_bounds__(256) lin_join_kernel(LinParams p, int main) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += s.get(e);
     }
+    if constexpr (PARTS == 3) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool bad = e < n && v[e] != v[e];
+        if (__any(bad)) v[e] = lin_again<EPI>(bad, i, j + e, v[e]);
+      }
+    }
     lin_by_kind<EPI>(p, [&](auto act, auto vec) {
       LinExtra<T> x;
       lin_extra<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x);
-      lin_finish<T, PARTS, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x, lin_bias<EPI>(p, j, p.bias_vec), v);
+      lin_finish<T, EPI, decltype(act)::value, decltype(vec)::value>(p, i, j, n, x, lin_bias<EPI>(p, j, p.bias_vec), v);
     });
   }
 }
