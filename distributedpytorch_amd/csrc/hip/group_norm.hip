@@ -905,7 +905,31 @@ static int gn_launch(const GnParams& p, bool bwd, hipStream_t s) {
   return dpa_launch_rc();
 }
 
+// Vectors that are written touch nothing else, and no activation that is written touches a vector that is read (which activations may
+// be one another the caller has checked).  Here because two dozen comparisons take the caller's language a microsecond.
+static bool gn_overlap(const GnParams& p, bool bwd, int es) {
+  struct Span { const char *a, *b; };
+  Span vout[2], vin[4], mout[2], min_[4];
+  int nvo = 0, nvi = 0, nmo = 0, nmi = 0;
+  const auto vec = [&](Span* to, int& n, const void* q, long long len) { if (q) to[n++] = {(const char*)q, (const char*)q + 4 * len}; };
+  const auto map = [&](Span* to, int& n, const void* q, long long cs) {
+    if (q) to[n++] = {(const char*)q, (const char*)q + (((long long)p.N * p.HW - 1) * cs + p.C) * es};
+  };
+  const long long ng = (long long)p.N * p.G;
+  vec(vin, nvi, p.gamma, p.C); vec(vin, nvi, p.beta, p.C);
+  vec(bwd ? vin : vout, bwd ? nvi : nvo, p.mean, ng); vec(bwd ? vin : vout, bwd ? nvi : nvo, p.rstd, ng);
+  if (bwd) { vec(vout, nvo, p.dgamma, p.C); vec(vout, nvo, p.dbeta, p.C); }
+  map(mout, nmo, p.y, p.y_cs); map(mout, nmo, p.dx, p.dx_cs); map(mout, nmo, p.dres, p.dres_cs);
+  map(min_, nmi, p.x, p.x_cs); map(min_, nmi, p.res, p.res_cs); map(min_, nmi, p.dy, p.dy_cs); map(min_, nmi, p.yv, p.yv_cs);
+  const auto any = [](const Span& s, const Span* o, int n) { for (int k = 0; k < n; ++k) if (s.a < o[k].b && o[k].a < s.b) return true; return false; };
+  for (int k = 0; k < nvo; ++k)
+    if (any(vout[k], vout + k + 1, nvo - k - 1) || any(vout[k], vin, nvi) || any(vout[k], mout, nmo) || any(vout[k], min_, nmi)) return true;
+  for (int k = 0; k < nmo; ++k) if (any(mout[k], vin, nvi)) return true;
+  return false;
+}
+
 DPA_API int dpa_gn_params_size() { return (int)sizeof(GnParams); }
 DPA_API int dpa_group_norm(const GnParams* p, int bwd, int f32, hipStream_t s) {
+  if (gn_overlap(*p, bwd, f32 ? 4 : 2)) return -1;
   return f32 ? gn_launch<float>(*p, bwd, s) : gn_launch<bf16_t>(*p, bwd, s);
 }

@@ -149,6 +149,20 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, ac
     return a, xs, dys, dxs, ys, rs, drs, vecs
 
 
+def group_norm_overlaps(name):
+    return ValueError(f"{name}: mean, rstd, dgamma or dbeta overlaps another argument, or an output overlaps gamma, beta, mean or rstd")
+
+
+def group_norm_vectors(name, outs, maps_out, vecs, maps):
+    """What csrc/hip/group_norm.hip: gn_overlap tests on the GPU, for the CPU form.  outs and vecs: vectors that are written and read;
+    maps_out and maps: spans of activations; None or NOTHING where there is none."""
+    spans = lambda ts: [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in ts if t is not None]  # noqa: E731
+    outs, vecs, maps_out, maps = spans(outs), spans(vecs), [(s[0], s[2]) for s in maps_out], [(s[0], s[2]) for s in maps]
+    pairs = [(a, b) for i, a in enumerate(outs) for b in outs[i + 1:] + vecs + maps_out + maps] + [(a, b) for a in maps_out for b in vecs]
+    if any(a[0] < b[1] and b[0] < a[1] for a, b in pairs):
+        raise group_norm_overlaps(name)
+
+
 # ------------------------------------------------------------------------------------------------ linear
 def linear_fprop(x, w, y, bias, act, addend, preact):
     """act's id, the spans of x, w, y, addend, preact, the address of bias"""
@@ -166,6 +180,8 @@ def linear_fprop(x, w, y, bias, act, addend, preact):
     ads = NOTHING if addend is None else mat_like(addend, "linear_fprop: addend", shape, dt, dev)
     zs = NOTHING if preact is None else mat_like(preact, "linear_fprop: preact", shape, dt, dev)
     b = 0 if bias is None else vec32(bias, "linear_fprop: bias", n, dev)
+    if b and (ys[0] - 4 * n < b < ys[2] or zs[0] - 4 * n < b < zs[2]):
+        raise ValueError(f"{name}: y or preact overlaps bias")
     apart(name, "y", y, ys, (("addend", addend, ads, True), ("x", x, xs, False), ("w", w, ws, False)))
     if preact is not None:
         apart(name, "preact", preact, zs, (("addend", addend, ads, True), ("x", x, xs, False), ("w", w, ws, False), ("y", y, ys, False)))
@@ -207,8 +223,8 @@ def linear_wgrad(dy, x, dw, db):
     dws = mat_like(dw, "linear_wgrad: dw", (n, k), torch.float32, dev)
     b = 0 if db is None else vec32(db, "linear_wgrad: db", n, dev)
     apart(name, "dw", dw, dws, (("dy", dy, dys, False), ("x", x, xs, False)))
-    if db is not None and not (b >= dws[2] or b + 4 * n <= dws[0]):
-        raise ValueError(f"{name}: db lies inside dw")
+    if b and (dws[0] - 4 * n < b < dws[2] or dys[0] - 4 * n < b < dys[2] or xs[0] - 4 * n < b < xs[2]):
+        raise ValueError(f"{name}: db overlaps dw, dy or x")
     return dys, xs, dws, b
 
 

@@ -151,7 +151,10 @@ def _gn_launch(stream, device, slab, coef, bwd, f32, head, tail):
     if slab + coef:
         ws = torch.empty(slab + coef, device=device, dtype=_F32)
         at = ws.data_ptr()
-    _lib().dpa_group_norm(_GN_PARAMS.pack(*head, at, at + 4 * slab, *tail), bwd, f32, stream)
+    rc = _lib().dpa_group_norm(_GN_PARAMS.pack(*head, at, at + 4 * slab, *tail), bwd, f32, stream)
+    if rc:
+        name = "group_norm_bwd" if bwd else "group_norm_fwd"
+        raise checks.group_norm_overlaps(name) if rc == -1 else native.KernelLaunchError(f"{name}: kernel launch failed with hipError_t {rc}")
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", residual=None):

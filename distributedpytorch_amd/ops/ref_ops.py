@@ -534,9 +534,10 @@ def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", resid
     """y = act((x - mean) * rstd * gamma + beta (+ residual)) for x [N, H, W, C] (fp32 or bf16, channel slices allowed), with
     the mean and 1 / sqrt(variance + eps) of each image's groups of C / groups channels, which are left in mean and rstd
     (fp32 [N, groups]) for the backward pass.  gamma, beta: fp32 [C].  act: "none", "relu", "silu" or "gelu".  y may be x
-    or residual itself."""
+    or residual itself; mean and rstd are apart from everything."""
     from . import checks
-    checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
+    _, xs, ys, rs, _ = checks.group_norm_fwd(x, gamma, beta, groups, y, mean, rstd, act, residual)
+    checks.group_norm_vectors("group_norm_fwd", (mean, rstd), (ys,), (gamma, beta), (xs, rs))
     if x.numel() == 0:
         return y
     t = _grouped(x.float(), groups)
@@ -557,9 +558,11 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
     """Gradients of group_norm_fwd: dx, dgamma and dbeta (fp32 [C], or None where they are not wanted) and dresidual (or
     None).  The activation's derivative is taken at values recomputed from x (and residual); for "relu" the stored output
     may be given as y instead, its sign is then the mask.  dresidual, the gradient of what stands under the activation, may be asked
-    for without a residual.  dx may be dy or x itself, dresidual may be dy, y or residual."""
+    for without a residual.  dx may be dy or x itself, dresidual may be dy, y or residual; dgamma and dbeta are apart
+    from everything."""
     from . import checks
-    checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
+    _, xs, dys, dxs, ys, rs, drs, _ = checks.group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma, dbeta, act, y, residual, dresidual)
+    checks.group_norm_vectors("group_norm_bwd", (dgamma, dbeta), (dxs, drs), (gamma, beta, mean, rstd), (xs, dys, ys, rs))
     if x.numel() == 0:
         for t in (dgamma, dbeta):
             if t is not None:

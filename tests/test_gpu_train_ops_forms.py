@@ -82,3 +82,12 @@ def test_group_norm(case, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_linear(case, dtype):
     cases.check_linear(case, dtype, "cuda")
+
+
+@pytest.mark.parametrize("name", sorted(forms.SHARED))
+def test_shared_memory_is_refused(name):
+    forms.check_shared(name, "cuda")
+
+
+def test_neighbours_in_a_buffer():
+    forms.check_neighbours("cuda")

@@ -112,3 +112,12 @@ def test_every_kernel_of_a_plan_has_a_case():
             n, k = (n + 7) // 8 * 8, (k + 7) // 8 * 8
         missing = linear_kernels(m, n, k) - there
         assert not missing, (missing, (m, n, k))
+
+
+@pytest.mark.parametrize("name", sorted(forms.SHARED))
+def test_shared_memory_is_refused(name):
+    forms.check_shared(name, "cpu")
+
+
+def test_neighbours_in_a_buffer():
+    forms.check_neighbours("cpu")

@@ -1,4 +1,5 @@
 """Forms of the group-norm and linear operators that each kernel of theirs has to take, shared by the CPU and GPU tests."""
+import pytest
 import torch
 
 from distributedpytorch_amd import ops
@@ -111,3 +112,67 @@ def check_infinities(case, dtype, device):
     want, err = O.product(dy.t(), x.t())
     O.close("dw", dw, want, err)
     O.close("db", db, dy.to(O.D).sum(0), (m + 8) * O.E * dy.to(O.D).abs().sum(0))
+
+
+def _norm(device, which, **kw):
+    a = dict(x=torch.randn(2, 4, 4, 8, device=device), dy=torch.randn(2, 4, 4, 8, device=device), gamma=torch.ones(8, device=device), beta=torch.zeros(8, device=device),
+             mean=torch.zeros(4, device=device), rstd=torch.ones(4, device=device), y=torch.empty(2, 4, 4, 8, device=device), dx=torch.empty(2, 4, 4, 8, device=device),
+             dg=torch.empty(8, device=device), db=torch.empty(8, device=device), res=None, dres=None)
+    for k, v in kw.items():
+        a[k] = v(a)
+    if which == "fwd":
+        ops.group_norm_fwd(a["x"], a["gamma"], a["beta"], 2, 1e-5, a["y"], a["mean"], a["rstd"], residual=a["res"])
+    else:
+        ops.group_norm_bwd(a["dy"], a["x"], a["gamma"], a["beta"], 2, a["mean"], a["rstd"], a["dx"], a["dg"], a["db"], residual=a["res"], dresidual=a["dres"])
+
+
+def _product(device, which, **kw):
+    a = dict(x=torch.randn(8, 8, device=device), w=torch.randn(8, 8, device=device), y=torch.empty(8, 8, device=device), z=torch.empty(8, 8, device=device),
+             bias=torch.randn(8, device=device), dy=torch.randn(8, 8, device=device), dw=torch.empty(8, 8, device=device), db=torch.empty(8, device=device))
+    for k, v in kw.items():
+        a[k] = v(a)
+    if which == "fprop":
+        ops.linear_fprop(a["x"], a["w"], a["y"], bias=a["bias"], act="gelu", preact=a["z"])
+    else:
+        ops.linear_wgrad(a["dy"], a["x"], a["dw"], db=a["db"])
+
+
+# arguments that share memory: what a kernel writes another block may still read
+SHARED = {
+    "mean is rstd": lambda d: _norm(d, "fwd", mean=lambda a: a["rstd"]),
+    "mean inside gamma": lambda d: _norm(d, "fwd", mean=lambda a: a["gamma"][2:6]),
+    "rstd inside y": lambda d: _norm(d, "fwd", rstd=lambda a: a["y"].view(-1)[8:12]),
+    "rstd inside x": lambda d: _norm(d, "fwd", rstd=lambda a: a["x"].view(-1)[-4:]),
+    "beta inside y": lambda d: _norm(d, "fwd", beta=lambda a: a["y"].view(-1)[16:24]),
+    "mean inside the residual": lambda d: _norm(d, "fwd", res=lambda a: a["x"].clone(), mean=lambda a: a["res"].view(-1)[:4]),
+    "dgamma is dbeta": lambda d: _norm(d, "bwd", dg=lambda a: a["db"]),
+    "dgamma is gamma": lambda d: _norm(d, "bwd", dg=lambda a: a["gamma"]),
+    "dbeta inside mean and beyond": lambda d: (lambda b: _norm(d, "bwd", mean=lambda a: b[:4], db=lambda a: b[3:11]))(torch.zeros(16, device=d)),
+    "dbeta inside dx": lambda d: _norm(d, "bwd", db=lambda a: a["dx"].view(-1)[:8]),
+    "dbeta inside dy": lambda d: _norm(d, "bwd", db=lambda a: a["dy"].view(-1)[:8]),
+    "gamma inside dx": lambda d: _norm(d, "bwd", gamma=lambda a: a["dx"].view(-1)[:8]),
+    "rstd inside dresidual": lambda d: _norm(d, "bwd", res=lambda a: a["x"].clone(), dres=lambda a: torch.empty_like(a["x"]), rstd=lambda a: a["dres"].view(-1)[:4]),
+    "bias inside y": lambda d: _product(d, "fprop", bias=lambda a: a["y"][3]),
+    "bias inside preact": lambda d: _product(d, "fprop", bias=lambda a: a["z"][7]),
+    "db inside dw": lambda d: _product(d, "wgrad", db=lambda a: a["dw"][0]),
+    "db inside dy": lambda d: _product(d, "wgrad", db=lambda a: a["dy"][7]),
+    "db inside x": lambda d: _product(d, "wgrad", db=lambda a: a["x"][0]),
+}
+
+
+def check_shared(name, device):
+    with pytest.raises(ValueError, match="overlaps"):
+        SHARED[name](device)
+
+
+def check_neighbours(device):
+    """Arguments that lie side by side in one buffer are apart."""
+    b = torch.zeros(4 + 4 + 8 + 8 + 256 + 8 + 8, device=device)
+    part = lambda lo, n: b[lo: lo + n]  # noqa: E731
+    y = part(24, 256).view(2, 4, 4, 8)
+    _norm(device, "fwd", mean=lambda a: part(0, 4), rstd=lambda a: part(4, 4), gamma=lambda a: part(8, 8), beta=lambda a: part(16, 8), y=lambda a: y)
+    _norm(device, "bwd", mean=lambda a: part(0, 4), rstd=lambda a: part(4, 4), gamma=lambda a: part(8, 8), beta=lambda a: part(16, 8), dx=lambda a: y,
+          dg=lambda a: part(280, 8), db=lambda a: part(288, 8))
+    c = torch.zeros(8 + 64 + 8, device=device)
+    _product(device, "fprop", bias=lambda a: c[:8], y=lambda a: c[8:72].view(8, 8))
+    _product(device, "wgrad", db=lambda a: c[72:], dw=lambda a: c[8:72].view(8, 8))
