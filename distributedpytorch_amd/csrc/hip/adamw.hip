@@ -11,9 +11,9 @@
 // Both kernels are bound by memory: one read and one write of every operand, 30 bytes a parameter with 32-bit
 // states and 18.25 with 8-bit ones (p 8, g 4, p16 2, states 16, or 4 and 0.25 of scales).  Operands that no kernel reads before the next step, larger together than
 // the caches, pass them by (nontemporal), and many short-lived blocks keep more requests in flight than 2048 long ones: 25.6
-// million parameters with p16 159 us in 2048 blocks with cached accesses, 147 in 16384, 133 (5.8 TB/s) with nontemporal ones.
+// million parameters with p16 159 us in 2048 blocks with cached accesses, 147 in 16384, 124 (6.2 TB/s) with nontemporal ones.
 // The 8-bit kernel computes some 110 instructions an element beside its bytes: 132.9 million parameters 528 us with
-// IEEE square roots, divisions and rounding by ldexp in 2048 blocks, 499 in 16384, 467 (5.2 TB/s) with the forms below; one
+// IEEE square roots, divisions and rounding by ldexp in 2048 blocks, 499 in 16384, 469 (5.2 TB/s) with the forms below; one
 // block a vector, or 4 elements a lane, was no faster (458, 487).
 #include "common.h"
 #include <algorithm>

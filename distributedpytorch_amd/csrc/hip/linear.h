@@ -206,8 +206,8 @@ template <int MT, int EPI> constexpr bool lin_sums() { return EPI == EPI_WGRAD &
 // the fragments of the NEXT phase from LDS.  The barrier stands before the last phase: behind it everyone's reads of the
 // buffer are done (registers hold what is left to multiply) and everyone's pieces of step s + 1 have landed.
 // P = 3: all three parts of both operands, each fragment read once for the six products of fp32 (P = 1 on parts walks over
-// them six times).  Half the LDS and DMA traffic, for tiles of which a CU has no second one to hide it behind; the larger
-// tile has no registers for it.  The fragments of step s + 1 are read while step s is multiplied.
+// them six times).  Half the LDS and DMA traffic, which is what bounds the smaller tiles (1021 x 1000 x 2048: the matrix pipe is busy
+// 33 % of the time); the larger tile has no registers for it.  The fragments of step s + 1 are read while step s is multiplied.
 template <typename T, int PARTS, int WM, int WN, int MT, int NT, int S, int P, int EPI>
 __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mfma_kernel(LinParams p) {
   constexpr bool AT = EPI == EPI_WGRAD, BT = EPI != EPI_FPROP;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(WM * WN * 64, P == 3 && MT > 2 ? 1 : 2) lin_mf
     // Sums of a's rows on the matrix pipe: a times ones, an accumulator for each row tile (one for all, with ones in a column
     // of each tile's own, would carry an infinity of one row, times zero, into others).  The waves that hold the same rows, WN in
     // each of the tiles of a row, take the steps in turn, so each pays in one step of `takers`.  bf16, 8192 x 4096 x 1024 with
-    // the bias gradient: 100 us, with a pass of its own over dy 110, without it 96; fp32, 2198 x 16 x 72: 13.9 and 13.4.
+    // the bias gradient: 92.2 us, without it 87.7, and a pass of its own over dy is 14; fp32, 2198 x 16 x 72: 14.2 and 13.8.
     constexpr bool SUMS = lin_sums<MT, EPI>();
     f32x4 sums[SUMS ? MT : 1];
 #pragma unroll

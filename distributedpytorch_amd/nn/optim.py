@@ -7,7 +7,7 @@ OIHW layout so the reference's `optimizer.load_state_dict` accepts it.
 
 "adamw" decouples the weight decay and applies it to matrices and filters only: biases and norm scales are a parameter group
 of their own, without decay, and `state_dict()` has the layout of torch.optim.AdamW over those two groups (decayed parameters
-first).  "adamw8" is the same with states of 8 bits (ops.adamw8_step): 2.03 bytes a parameter instead of 8.  It is saved as the
+first).  "adamw8" is the same with states of 8 bits (ops.adamw8_step): 2.125 bytes a parameter instead of 8.  It is saved as the
 32-bit values its states stand for, with the scales as entries of the first parameter group; loading rounds to nearest,
 which gives the same codes again.  A checkpoint of one kind loads into the other.
 """

@@ -185,16 +185,17 @@ _FPROP, _DGRAD, _WGRAD = 0, 1, 2          # csrc/hip/linear.h
 def _plan(rows, cols, k, f32):
     """(tile of lin_tile, splits of the reduction).  The largest tile that still fills the chip: 256 x 256 runs one block on
     each of the 256 CUs, 128 x 128 two (or one with four steps in LDS), 64 x 64 two.  Measured on both sides, us:
-      256 x 256 below K = 384 pays more for its epilogue than it saves (2909 x 6280 x 192: 28.7, 128 x 128 23.8; 10382 x 5456
-        x 480: 80.6, 94.1); fp32 walks over K six times and has no such bound;
-      128 x 128 from 140 tiles on (1433 x 1872 x 2640, 180 tiles: 36.6, 64 x 64 44.1; 715 x 560 x 1504, 30 tiles: 19, 13.4);
-        two blocks a CU above 256 tiles (6306 x 1112 x 736: 22.6, one 28.8), four steps in LDS below (2048^3: 28.6, 30.4);
+      256 x 256 below K = 384 pays more for its epilogue than it saves (2909 x 6280 x 192: 29.1, 128 x 128 23.2; 10382 x 5456
+        x 480: 84.2, 90.2); fp32 walks over K six times and has no such bound;
+      128 x 128 from 140 tiles on (1433 x 1872 x 2640, 180 tiles: 31.2, 64 x 64 37.6; 715 x 560 x 1504, 30 tiles: 20.4, 11.7);
+        two blocks a CU above 256 tiles (6306 x 1112 x 736: 21.3, one 25.8), four steps in LDS below (2048^3: 25.4, 30.0);
       fp32 in tiles of 128 x 128 has one block a CU, so the last round has to be well filled (688 x 5688 x 888, 270 tiles: 91.9,
         64 x 64 82.3), and a long reduction is split over it (976 x 744 x 5741: 84 in five, 64 x 64 125 whole and 123 in two);
         up to 512 elements a part 64 x 64 in one round needs no split and no launch to join it (1021 x 1000 x 2048: 44.0, 128 x
         128 in four 45.8; 900 x 700 x 1600: 37.9, 51.7 in three);
-      a split costs a pass over its partial products and pays from 512 elements a part on (3119 x 280 x 624: 9.6 whole, 15.8
-        in two; 784 x 184 x 4670: 15.7 in six, 25 whole; 792 x 1424 x 6161 in 128 x 128: 36.8 in six, 57.8 in whole 64 x 64),
+      a split costs a pass over its partial products and pays from 512 elements a part on (3119 x 280 x 624: 7.9 whole, 14.6
+        in two; a weight gradient of 784 x 184 x 4670: 14.7 in six, 28.7 whole, of 792 x 1424 x 6161 in 128 x 128: 34.7 in six, 55.4
+        in whole 64 x 64),
         in fp32 with few tiles from 128 on (176 x 248 x 571: 13.4 in four, 15.7 whole), as long as every part has a CU of its own: two
         blocks share one's LDS traffic (256 x 1000 x 2048, 64 tiles: 28.2 in four, 30.5 in eight; 900 x 900 x 1400, 225 tiles:
         44.0 whole, 52.5 in two; 700 x 700 x 2048, 121 tiles: 37.0 in two, 40.3 in four)."""
@@ -226,7 +227,8 @@ def _linear(stream, epi, t_a, a, t_b, b, rows, cols, k, vec, act=0, out=checks.N
     parts = 3 if f32 else 1
     need = ld_a = ld_b = a_part = b_part = pack_a = pack_b = ws = sums = db_out = db_slab = takers = db_splits = 0
     if epi == _FPROP and rows <= (64 if f32 else 32) and cols < 1 << 27 and ok_a and ok_b and not (k * es) & 15:
-        # (a launch has fewer than 2^32 threads, 32 for a column; 32 rows x 4096 x 4096 in bf16: 14.6 us, in 64 x 64 tiles 15.2; 64 rows: 21.5 and 15.2.  fp32, 64 rows: 48 and 60)
+        # (a launch has fewer than 2^32 threads, 32 for a column; 32 rows x 4096 x 4096 in bf16: 15.0 us, in 64 x 64 tiles 18.8; 64 rows: 21.6 and 19.7.
+        # fp32, 64 rows: 47.9 and 56.8)
         tile, splits = -1, 1
     else:
         tile, splits = _plan(rows, cols, k, f32)
