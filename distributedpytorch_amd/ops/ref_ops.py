@@ -525,6 +525,10 @@ def _act_slope(u, act):
     return torch.ones_like(u)
 
 
+# (sums over pixels and rows in 64 bits: over dimensions that are not innermost torch adds one value behind another on the CPU)
+_SUM = torch.float64
+
+
 def _grouped(t, groups):
     n, h, w, c = t.shape
     return t.reshape(n, h * w, groups, c // groups)
@@ -541,9 +545,9 @@ def group_norm_fwd(x, gamma, beta, groups, eps, y, mean, rstd, act="none", resid
     if x.numel() == 0:
         return y
     t = _grouped(x.float(), groups)
-    mu = t.mean((1, 3))
+    mu = t.mean((1, 3), dtype=_SUM).float()
     d = t - mu[:, None, :, None]
-    rs = torch.rsqrt((d * d).mean((1, 3)) + eps)
+    rs = torch.rsqrt((d * d).mean((1, 3), dtype=_SUM) + eps).float()
     u = (d * rs[:, None, :, None]).reshape(x.shape) * gamma + beta
     if residual is not None:
         u = u + residual.float()
@@ -580,11 +584,12 @@ def group_norm_bwd(dy, x, gamma, beta, groups, mean, rstd, dx, dgamma=None, dbet
         u = xhat.reshape(x.shape) * gamma + beta
         dz = dz * _act_slope(u if residual is None else u + residual.float(), act)
     t = _grouped(dz * gamma, groups)
-    out = rs * (t - t.mean((1, 3), keepdim=True) - xhat * (t * xhat).mean((1, 3), keepdim=True))
+    c1, c2 = (v.mean((1, 3), keepdim=True, dtype=_SUM).float() for v in (t, t * xhat))
+    out = rs * (t - c1 - xhat * c2)
     if dgamma is not None:
-        dgamma.copy_((_grouped(dz, groups) * xhat).sum((0, 1)).reshape(-1))
+        dgamma.copy_((_grouped(dz, groups) * xhat).sum((0, 1), dtype=_SUM).reshape(-1))
     if dbeta is not None:
-        dbeta.copy_(dz.sum((0, 1, 2)))
+        dbeta.copy_(dz.sum((0, 1, 2), dtype=_SUM))
     if dresidual is not None:
         dresidual.copy_(dz)
     dx.copy_(out.reshape(x.shape))
@@ -628,7 +633,7 @@ def linear_wgrad(dy, x, dw, db=None, accumulate=False):
     """dw = dy^T x (fp32 [out, in]) and db = the column sums of dy (fp32 [out]); accumulate adds to what they hold."""
     from . import checks
     checks.linear_wgrad(dy, x, dw, db)
-    w, b = dy.float().t() @ x.float(), dy.float().sum(0)
+    w, b = dy.float().t() @ x.float(), dy.sum(0, dtype=_SUM).float()
     if accumulate:
         dw.add_(w)
         if db is not None:

@@ -91,3 +91,12 @@ def test_shared_memory_is_refused(name):
 
 def test_neighbours_in_a_buffer():
     forms.check_neighbours("cuda")
+
+
+@pytest.mark.parametrize("case", forms.FAR, ids=str)
+def test_means_far_from_zero(case):
+    forms.check_far_means(case, "cuda")
+
+
+def test_sums_over_many_rows():
+    forms.check_long_sums("cuda")

@@ -121,3 +121,12 @@ def test_shared_memory_is_refused(name):
 
 def test_neighbours_in_a_buffer():
     forms.check_neighbours("cpu")
+
+
+@pytest.mark.parametrize("case", forms.FAR, ids=str)
+def test_means_far_from_zero(case):
+    forms.check_far_means(case, "cpu")
+
+
+def test_sums_over_many_rows():
+    forms.check_long_sums("cpu")

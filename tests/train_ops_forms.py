@@ -176,3 +176,45 @@ def check_neighbours(device):
     c = torch.zeros(8 + 64 + 8, device=device)
     _product(device, "fprop", bias=lambda a: c[:8], y=lambda a: c[8:72].view(8, 8))
     _product(device, "wgrad", db=lambda a: c[72:], dw=lambda a: c[8:72].view(8, 8))
+
+
+# (n, h, w, c, groups): vector kernels in one pass and two, one channel a lane, any layout; up to 104 values a thread
+FAR = [(4, 28, 28, 512, 32), (2, 7, 7, 64, 8), (2, 112, 112, 64, 32), (2, 13, 13, 30, 3), (2, 40, 40, 30, 3), (1, 64, 64, 48, 4)]
+
+
+def check_far_means(case, device):
+    """Means of 330 with a spread of 0.1.  m values summed one behind another round E (1 + ... + m) of their size, so E m / 2 of the sum:
+    52 for 104 values a thread, as many again where the partial sums of a group's threads are added (at most 128), some 20 for
+    trees, joins and the division.  The second moment holds that error squared, and 512 roundings of its own."""
+    n, h, w, c, groups = case
+    gen = torch.Generator().manual_seed(h + c)
+    x = torch.randn(n, h, w, c, generator=gen) * 0.1 + 330 + 0.002 * torch.arange(c)
+    gamma, beta = torch.rand(c, generator=gen) + 0.5, torch.randn(c, generator=gen)
+    xd, y, (mean, rstd) = x.to(device), torch.empty(n, h, w, c, device=device), torch.empty(2, n, groups, device=device)
+    ops.group_norm_fwd(xd, gamma.to(device), beta.to(device), groups, 1e-5, y, mean, rstd)
+    t = O.grouped(x, groups)
+    mu = t.mean((1, 3))
+    d = t - mu[:, None, :, None]
+    rs = 1 / ((d * d).mean((1, 3)) + 1e-5).sqrt()
+    off = 136 * O.E * mu.abs()
+    e_rs = rs * (0.5 * (off * rs) ** 2 + 544 * O.E)
+    O.close("mean", mean, mu, off)
+    O.close("rstd", rstd, rs, e_rs)
+    hat = (d * rs[:, None, :, None]).reshape(x.shape)
+    e = gamma.to(O.D) * (hat.abs() * O._per(e_rs / rs, x, groups) + O._per(off * rs, x, groups)) + 8 * O.E * (hat.abs() + beta.abs())
+    O.close("y", y, hat * gamma.to(O.D) + beta.to(O.D), e)
+
+
+def check_long_sums(device):
+    """Parameter gradients over 300 thousand pixels and rows, of one sign: at most 2^13 roundings in a row."""
+    gen = torch.Generator().manual_seed(3)
+    n, h, w, c, groups = 1, 600, 500, 8, 2
+    x, dy = torch.randn(n, h, w, c, generator=gen), torch.rand(n, h, w, c, generator=gen) + 0.5
+    xd, y, (mean, rstd), (dg, db) = x.to(device), torch.empty(n, h, w, c, device=device), torch.empty(2, n, groups, device=device), torch.empty(2, c, device=device)
+    ga, be = torch.ones(c, device=device), torch.zeros(c, device=device)
+    ops.group_norm_fwd(xd, ga, be, groups, 1e-5, y, mean, rstd)
+    ops.group_norm_bwd(dy.to(device), xd, ga, be, groups, mean, rstd, y, dg, db)
+    O.close("dbeta", db, dy.to(O.D).sum((0, 1, 2)), 2 ** 13 * O.E * dy.to(O.D).sum((0, 1, 2)))
+    dw, db = torch.empty(c, c, device=device), torch.empty(c, device=device)
+    ops.linear_wgrad(dy.view(-1, c).to(device), xd.view(-1, c), dw, db)
+    O.close("db", db, dy.to(O.D).sum((0, 1, 2)), 2 ** 13 * O.E * dy.to(O.D).sum((0, 1, 2)))
